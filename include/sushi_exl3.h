@@ -313,6 +313,83 @@ sx_status sx_moe_static_scratch(sx_stream stream, const sx_bank* bank, const sx_
 /* The size of sx_moe_static_scratch's buffer in bytes. */
 size_t sx_moe_static_scratch_bytes(void);
 
+/* ------------------------------------------------------------------ 4-bit key/value cache
+ * What stands between a layer's query/key/value projections and its output projection at serving
+ * time: a paged cache that holds keys and values in 4 bits, the block tables of a step, and the
+ * attention that reads the cache.  No counterpart in the reference's path (its attention runs in
+ * the Zig host's own engine).
+ *
+ * Format.  A token's key (and value) of one head is head_dim channels in groups of 64.  A group x
+ * is held as 4-bit codes with an F16 minimum m and step s:
+ *   m = f16(min x), s = f16((max x - min x) * (1/15)),  code = clamp(rint((x - m) / s), 0, 15)
+ * (0 where s = 0), and stands for code * s + m: 4.5 bits a channel.  Finite inputs past F16's range
+ * count as its largest value; a group with a NaN or an infinity is held as NaN.
+ * The pool is [pages][kv_heads] blocks of sx_kv4_block_bytes(head_dim, page_size) bytes; a block
+ * holds page_size tokens of one head, keys and values, and its inner order is the library's own.
+ * Place ("slot") p is token p % page_size of page p / page_size. */
+typedef struct sx_kv4 {
+    void* pool;          /* device, 16-byte aligned, pages * kv_heads * sx_kv4_block_bytes() bytes */
+    int32_t pages;
+    int32_t kv_heads;
+    int32_t head_dim;    /* 64, 128 or 256 */
+    int32_t page_size;   /* tokens a page: 16, 32, 64, 128 or 256 */
+} sx_kv4;
+
+/* Bytes of one page's block of one head; 0 for a head_dim or page_size outside the format. */
+size_t sx_kv4_block_bytes(int32_t head_dim, int32_t page_size);
+
+/* The block tables of one serving step, from request lengths that are on the device.  Request b
+ * holds ctx_lens[b] cached tokens and adds new_lens[b] (either may be 0; a negative length counts
+ * as 0).  table [requests] rows of table_width page ids, table_stride entries apart: row b's first
+ * ceil(ctx/page_size) entries are its pages so far; the entries for its new tokens are filled in
+ * from the stack of free pages free_pages[0 .. free_count[0]), in request order, taking from the
+ * stack's end (-1 once the stack is used up, and free_left[0] is then negative: the shortage).
+ * Entries past table_width are not allocated.  Outputs (none may overlap the inputs; the lengths
+ * and the stack are left as they are, so a step can be prepared again):
+ *   kv_lens [requests] = ctx + new;   cu_q [requests + 1], the running sum of new_lens;
+ *   slots [tokens] and positions [tokens]: place and position of token i of the step (slot -1
+ *   without a page; -1 and 0 past the last request's tokens);   free_left [1].
+ * requests 1..16384, tokens >= 0 (the capacity of slots and positions); ctx + new and the sum of
+ * new below 2^31. */
+sx_status sx_block_tables(sx_stream stream, const int32_t* ctx_lens, const int32_t* new_lens, int32_t requests,
+                          int32_t page_size, int32_t* table, int32_t table_width, int64_t table_stride,
+                          const int32_t* free_pages, const int32_t* free_count, int32_t tokens, int32_t* kv_lens,
+                          int32_t* cu_q, int64_t* slots, int32_t* positions, int32_t* free_left);
+
+/* Writes the keys and values of `tokens` tokens into places slots[i] (a place outside the pool, -1
+ * for one, is skipped; two tokens must not name one place).  k and v [tokens][kv_heads][head_dim]
+ * of `dtype` (BF16, F16 or F32), channels contiguous, the strides between tokens and heads in
+ * elements (so views of a fused projection's output need no copy). */
+sx_status sx_kv4_write(sx_stream stream, const sx_kv4* cache, const void* k, int64_t k_token_stride,
+                       int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                       sx_dtype dtype, int32_t tokens, const int64_t* slots);
+
+/* The held keys and values of `tokens` places, rounded to `dtype`: k and v contiguous
+ * [tokens][kv_heads][head_dim]; zeros for a place outside the pool. */
+sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slots, int32_t tokens, sx_dtype dtype,
+                      void* k, void* v);
+
+/* Attention over the cache, for single tokens, drafted tokens and prompt chunks, mixed in one call.
+ * Request b's rows are q rows cu_q[b] .. cu_q[b+1] (q_len of them, at most max_q); its keys are
+ * positions 0 .. kv_lens[b], the step's own tokens last (written before this call).  Row i stands at
+ * position p = kv_lens[b] - q_len + i and sees positions <= p, and > p - window when window > 0:
+ *   out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j      (k, v of head h * kv_heads / heads)
+ * in f32, with the probabilities times each step s rounded to F16 before the product with the
+ * codes.  A row that sees nothing (kv_len 0, or q_len > kv_len), and rows past cu_q[requests], are 0.
+ * Positions whose page id is outside the pool, or past table_width pages, count as unseen.
+ * q [tokens][heads][head_dim] with strides in elements, channels contiguous; out contiguous; both of
+ * `dtype`, BF16 or F16 (SX_ERR_BAD_DTYPE for F32: the products take 16-bit operands).  heads is a
+ * multiple of kv_heads; scale finite.  workspace: sx_kv4_attention_workspace_bytes(...) bytes,
+ * 16-byte aligned, ZEROED before its first use; every call leaves what has to be zero at zero, also
+ * for calls of other sizes.  Calls that may run at the same time need their own. */
+size_t sx_kv4_attention_workspace_bytes(const sx_kv4* cache, int32_t requests, int32_t tokens, int32_t heads,
+                                        int32_t max_q);
+sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q, int64_t q_token_stride,
+                           int64_t q_head_stride, sx_dtype dtype, int32_t tokens, int32_t heads, const int32_t* cu_q,
+                           const int32_t* kv_lens, const int32_t* table, int32_t requests, int32_t table_width,
+                           int64_t table_stride, int32_t max_q, float scale, int32_t window, void* out, void* workspace,
+                           size_t workspace_bytes);
+
 /* ------------------------------------------------------------------ expert parallel
  * The routed layer with its experts sharded over `world` GPUs (one process or thread per GPU):
  * rank g holds experts [g*E/world, (g+1)*E/world) of an E-expert layer as a local bank of E/world

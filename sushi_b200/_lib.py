@@ -45,8 +45,19 @@ class SxRagged(ctypes.Structure):
     ]
 
 
+class SxKv4(ctypes.Structure):
+    _fields_ = [
+        ("pool", ctypes.c_void_p),
+        ("pages", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
+_L = ctypes.c_int64
 _SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes); every symbol include/sushi_exl3.h declares.
@@ -75,6 +86,13 @@ SIGNATURES = {
                            _P, _SZ]),
     "sx_moe_static_scratch": (_I, [_P, ctypes.POINTER(SxBank), ctypes.POINTER(SxDecode), _P, _I, _I, _P, _P, _I, _P, _P, _I, _P]),
     "sx_moe_static_scratch_bytes": (_SZ, []),
+    "sx_kv4_block_bytes": (_SZ, [_I, _I]),
+    "sx_block_tables": (_I, [_P, _P, _P, _I, _I, _P, _I, _L, _P, _P, _I, _P, _P, _P, _P, _P]),
+    "sx_kv4_write": (_I, [_P, ctypes.POINTER(SxKv4), _P, _L, _L, _P, _L, _L, _I, _I, _P]),
+    "sx_kv4_read": (_I, [_P, ctypes.POINTER(SxKv4), _P, _I, _I, _P, _P]),
+    "sx_kv4_attention_workspace_bytes": (_SZ, [ctypes.POINTER(SxKv4), _I, _I, _I, _I]),
+    "sx_kv4_attention": (_I, [_P, ctypes.POINTER(SxKv4), _P, _L, _L, _I, _I, _I, _P, _P, _P, _I, _I, _L, _I,
+                              ctypes.c_float, _I, _P, _P, _SZ]),
     "sx_ep_unique_id": (_I, [_P]),
     "sx_ep_init": (_I, [_P, _I, _I, _P]),
     "sx_ep_destroy": (_I, [_P]),
