@@ -5,25 +5,9 @@
 #include <algorithm>
 #include <cmath>
 
-#include "sx_kv4.cuh"
+#include "sx_kv4_attn.cuh"
 
 namespace sx {
-
-struct Kv4AttnArgs {
-    const uint8_t* pool;
-    int pages, kv_heads, page_size, shift;
-    const void* q;
-    long long qts, qhs;
-    void* out;
-    int dt, tokens, heads;
-    const int* cu_q;
-    const int* kv_lens;
-    const int* table;
-    int requests, width;
-    long long tstride;
-    float scale;
-    int window;
-};
 
 constexpr int kAttnWarps = 4;
 
@@ -41,9 +25,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_rows_kernel(Kv4AttnA
     int b = -1;
     for (int i = 0; i < a.requests; i++)
         if (row >= a.cu_q[i] && row < a.cu_q[i + 1]) b = i;
-    if (b >= 0) {
+    if (b < 0 || (a.cu_q[b + 1] - a.cu_q[b]) * (long long)a.group <= a.max_cols) return;  // the streaming kernel's
+    {
         for (int c = lane; c < D; c += 32)
-            qs[warp][c] = load_act(a.q, row * a.qts + head * a.qhs + c, a.dt) * a.scale;
+            qs[warp][c] = load_act(a.q, row * a.qts + head * a.qhs + c, a.dt) * a.scale_log2;
         __syncwarp();
         const int kv = min(a.kv_lens[b], a.width * a.page_size);
         const int pos = a.kv_lens[b] - (a.cu_q[b + 1] - a.cu_q[b]) + row - a.cu_q[b];
@@ -78,8 +63,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_rows_kernel(Kv4AttnA
             if (!__any_sync(0xffffffffu, gran != nullptr)) continue;
             // A NaN score is passed over by fmaxf and lands in the sums.
             const float mnew = fmaxf(m, top), mref = mnew == -CUDART_INF_F ? 0.0f : mnew;
-            const float corr = m == -CUDART_INF_F ? 0.0f : expf(m - mref);
-            const float p = gran ? expf(s - mref) : 0.0f;
+            const float corr = m == -CUDART_INF_F ? 0.0f : ex2(m - mref);
+            const float p = gran ? ex2(s - mref) : 0.0f;
             float sum = p;
 #pragma unroll
             for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -112,12 +97,21 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv4_attn_rows_kernel(Kv4AttnA
 
 using namespace sx;
 
+namespace {
+
+// The workspace: a counter a CTA, then two partial slots a CTA of 16 columns.
+size_t counters_bytes() { return (size_t)kv4_max_ctas() * sizeof(int); }
+size_t part_bytes(int D) { return (size_t)kv4_max_ctas() * 2 * 16 * (D + 2) * sizeof(float); }
+
+}  // namespace
+
 extern "C" {
 
 size_t sx_kv4_attention_workspace_bytes(const sx_kv4* cache, int32_t requests, int32_t tokens, int32_t heads,
                                         int32_t max_q) {
-    (void)cache, (void)requests, (void)tokens, (void)heads, (void)max_q;
-    return 16;
+    (void)requests, (void)tokens, (void)heads, (void)max_q;
+    if (!cache || !kv4_dim_ok(cache->head_dim)) return 0;
+    return counters_bytes() + part_bytes(cache->head_dim);
 }
 
 sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q, int64_t q_token_stride,
@@ -133,7 +127,7 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
         return SX_ERR_BAD_SHAPE;
     if (tokens == 0) return SX_OK;
     if (!q || !cu_q || !kv_lens || !table || !out || !workspace) return SX_ERR_NULL_POINTER;
-    if (reinterpret_cast<uintptr_t>(workspace) % 16) return SX_ERR_BAD_SHAPE;
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 || reinterpret_cast<uintptr_t>(out) % 16) return SX_ERR_BAD_SHAPE;
     if (workspace_bytes < sx_kv4_attention_workspace_bytes(cache, requests, tokens, heads, max_q))
         return SX_ERR_WORKSPACE_TOO_SMALL;
     Kv4AttnArgs a = {};
@@ -144,10 +138,19 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     a.out = out, a.dt = dtype, a.tokens = tokens, a.heads = heads;
     a.cu_q = cu_q, a.kv_lens = kv_lens, a.table = table;
     a.requests = requests, a.width = table_width, a.tstride = table_stride;
-    a.scale = scale, a.window = window;
+    a.group = heads / cache->kv_heads;
+    a.qvec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
+    a.scale_log2 = (float)(scale * 1.4426950408889634), a.window = window;
+    const long long most = (long long)max_q * a.group;  // columns a key head, of any request
+    a.max_cols = a.group > 8 || (most > 8 && most <= 16) ? 16 : 8;
+    a.count = static_cast<int*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + counters_bytes());
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e = kv4_stream_launch(a, cache->head_dim, s);
+    if (e != cudaSuccess) return cuda_status(e, "kv4_attention stream launch");
+    if (most <= a.max_cols) return SX_OK;
     const long long items = (long long)tokens * heads;
     const unsigned grid = (unsigned)((items + kAttnWarps - 1) / kAttnWarps);
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (cache->head_dim == 64) kv4_attn_rows_kernel<64><<<grid, kAttnWarps * 32, 0, s>>>(a);
     else if (cache->head_dim == 128) kv4_attn_rows_kernel<128><<<grid, kAttnWarps * 32, 0, s>>>(a);
     else kv4_attn_rows_kernel<256><<<grid, kAttnWarps * 32, 0, s>>>(a);

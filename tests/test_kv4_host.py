@@ -80,6 +80,7 @@ def test_cache_refusals(L, kw, want):
         (dict(out=None), "SX_ERR_NULL_POINTER"),
         (dict(ws=None), "SX_ERR_NULL_POINTER"),
         (dict(ws=FAKE + 8), "SX_ERR_BAD_SHAPE"),
+        (dict(out=FAKE + 2), "SX_ERR_BAD_SHAPE"),
         (dict(nbytes=1), "SX_ERR_WORKSPACE_TOO_SMALL"),
         (dict(tokens=0, q=None), "SX_OK"),
     ],
