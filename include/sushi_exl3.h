@@ -322,8 +322,8 @@ size_t sx_moe_static_scratch_bytes(void);
  * Format.  A token's key (and value) of one head is head_dim channels in groups of 64.  A group x
  * is held as 4-bit codes with an F16 minimum m and step s:
  *   m = f16(min x), s = f16((max x - min x) * (1/15)),  code = clamp(rint((x - m) / s), 0, 15)
- * (0 where s = 0), and stands for code * s + m: 4.5 bits a channel.  Finite inputs past F16's range
- * count as its largest value; a group with a NaN or an infinity is held as NaN.
+ * (0 where s = 0), and stands for code * s + m: 4.5 bits a channel.  Finite inputs past
+ * +-57344 count as that (held values stay within F16); a group with a NaN or an infinity is held as NaN.
  * The pool is [pages][kv_heads] blocks of sx_kv4_block_bytes(head_dim, page_size) bytes; a block
  * holds page_size tokens of one head, keys and values, and its inner order is the library's own.
  * Place ("slot") p is token p % page_size of page p / page_size. */
@@ -374,11 +374,11 @@ sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slot
  * positions 0 .. kv_lens[b], the step's own tokens last (written before this call).  Row i stands at
  * position p = kv_lens[b] - q_len + i and sees positions <= p, and > p - window when window > 0:
  *   out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j      (k, v of head h * kv_heads / heads)
- * in f32, with the probabilities times each step s rounded to F16 before the product with the
- * codes.  A row that sees nothing (kv_len 0, or q_len > kv_len), and rows past cu_q[requests], are 0.
+ * with f32 sums; operands of the products (query, probability times step, or held key and value where
+ * a request has many rows) are rounded to F16.  A row that sees nothing (kv_len 0, or q_len > kv_len), and rows past cu_q[requests], are 0.
  * Positions whose page id is outside the pool, or past table_width pages, count as unseen.
- * q [tokens][heads][head_dim] with strides in elements, channels contiguous; out contiguous; both of
- * `dtype`, BF16 or F16 (SX_ERR_BAD_DTYPE for F32: the products take 16-bit operands).  heads is a
+ * q [tokens][heads][head_dim] with strides in elements, channels contiguous; out contiguous and
+ * 16-byte aligned; both of `dtype`, BF16 or F16 (SX_ERR_BAD_DTYPE for F32: the products take 16-bit operands).  heads is a
  * multiple of kv_heads; scale finite.  workspace: sx_kv4_attention_workspace_bytes(...) bytes,
  * 16-byte aligned, ZEROED before its first use; every call leaves what has to be zero at zero, also
  * for calls of other sizes.  Calls that may run at the same time need their own. */

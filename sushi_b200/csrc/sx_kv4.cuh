@@ -23,6 +23,8 @@
 namespace sx {
 
 constexpr int kKvGroup = 64;    // channels that share a step and a minimum
+// Inputs past this count as it: 15 s + m, with s and m rounded to F16, then stays within F16.
+constexpr float kKvLargest = 57344.0f;
 constexpr int kKvGranule = 16;  // tokens of one contiguous piece of a block
 
 __host__ __device__ constexpr int kv4_granule_bytes(int D) { return kKvGranule * (D + 8 * (D / kKvGroup)); }

@@ -63,5 +63,8 @@ __device__ __forceinline__ uint32_t pack_act2(float a, float b, int dt) {
 // The streaming kernel (sx_kv4_stream.cu).  kv4_max_ctas: CTAs no launch of it passes.
 inline int kv4_max_ctas() { return 4 * sm_count(); }
 cudaError_t kv4_stream_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream);
+// The tile kernel (sx_kv4_tile.cu), one CTA an SM; floats of one of its two partial slots a CTA.
+size_t kv4_tile_part_floats(int D);
+cudaError_t kv4_tile_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream);
 
 }  // namespace sx

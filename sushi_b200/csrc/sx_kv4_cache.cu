@@ -180,11 +180,11 @@ __global__ void __launch_bounds__(kKvThreads) kv4_write_kernel(KvIoArgs a) {
     float x[8];
     load8(a.src[kv], t * a.ts[kv] + h * a.hs[kv] + piece * 8, a.dt, a.vec, x);
     bool bad = false;
-    float lo = 65504.0f, hi = -65504.0f;
+    float lo = kKvLargest, hi = -kKvLargest;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         bad |= !(fabsf(x[j]) <= 3.402823466e38f);
-        x[j] = fminf(fmaxf(x[j], -65504.0f), 65504.0f);
+        x[j] = fminf(fmaxf(x[j], -kKvLargest), kKvLargest);
         lo = fminf(lo, x[j]);
         hi = fmaxf(hi, x[j]);
     }

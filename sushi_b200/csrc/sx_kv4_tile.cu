@@ -1,0 +1,761 @@
+// Attention over the 4-bit cache for requests of many rows (prompt chunks, long drafts, many query
+// heads a key head) on the tensor cores.
+//
+// A unit is one request, key head and block of 128 MT (row, query head) pairs, MT = 2 (1 at D = 256,
+// whose output accumulator takes half the tensor memory).  Per tile of NK keys:
+//   S = Q K^T  (tcgen05, M = 128, N = NK, both from shared memory, f32 in tensor memory)
+//   P = exp2(c S - ref) by one thread a row, F16, over S's columns in tensor memory
+//   O += P V   (tcgen05, A = P from tensor memory, B = V from shared memory)
+// Four warps widen the codes to F16 tiles, key and value alike (code * s + m, rounded once: one word
+// of eight codes is one 16-byte chunk), from granules that bulk copies bring.  Eight consecutive
+// channels lie in the order of a word's nibble pairs (0 4 1 5 2 6 3 7), in Q and K alike, and in O's
+// columns.  Keys are K-major (rows of 64 channels, 128-byte swizzle); values have the same image,
+// read as the N-major operand.  The two row tiles take turns: one's softmax runs under the other's
+// products.  The reference moves only when a score passes it by 2^8 (P's best at 2^7, at most 2^15).
+//
+// Work: the units' tiles laid end to end and cut into equal runs, one a CTA (one CTA an SM), so
+// causal lengths balance and few long rows are split; a unit of several CTAs is joined by the last
+// to arrive, in CTA order.  Every wait is bounded (sx_common.cuh).
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include "sx_gemm_impl.cuh"
+#include "sx_kv4_attn.cuh"
+
+namespace sx {
+
+constexpr int kTlDeqWarps = 4;
+
+template <int D>
+struct TileLayout {
+    static constexpr int G = D / kKvGroup;
+    static constexpr int MT = D == 256 ? 1 : 2;
+    static constexpr int NK = D == 256 ? 64 : 128;
+    static constexpr int KST = 2, VST = D == 256 ? 1 : 2;
+    static constexpr int ROWS = 128 * MT;
+    static constexpr int SM_WARPS = 4 * MT;
+    static constexpr int THREADS = (SM_WARPS + kTlDeqWarps + 1) * 32;
+    static constexpr int GB = kv4_granule_bytes(D);
+    static constexpr int GPW = NK / kKvGranule / kTlDeqWarps;  // granules a warp a tile
+    static constexpr int RING = D == 128 ? 3 : (D == 64 ? 4 : 2);
+    static constexpr int Q_TILE = 128 * D * 2;
+    static constexpr int KV_TILE = NK * D * 2;
+    static constexpr int SUB = NK * 128;  // bytes of 64 channels of a key tile
+    static constexpr int Q = 0;
+    static constexpr int K = Q + MT * Q_TILE;
+    static constexpr int V = K + KST * KV_TILE;
+    static constexpr int RAW = V + VST * KV_TILE;
+    static constexpr int BAD = RAW + kTlDeqWarps * RING * GB;  // [VST][G][NK / 16] u16
+    static constexpr int BAR = (BAD + VST * G * (NK / 16) * 2 + 15) / 16 * 16;
+    static constexpr int NBAR = kTlDeqWarps * RING + 2 * KST + 2 * VST + 2 + 2 + 2 + 1;
+    static constexpr int TOTAL = BAR + NBAR * 8;
+    static constexpr int ALLOC = TOTAL + 1024;
+    static constexpr int S_COL = 0;  // two S tiles of NK columns
+    static constexpr int O_COL = 256;
+    static_assert(ALLOC <= 227 * 1024, "fits a CTA");
+};
+
+// Block u of a request's (row, head) pairs: n tiles of keys from position lo.
+struct TileUnit {
+    int e0, rows;  // pairs [e0, e0 + rows)
+    int lo, n;
+};
+
+template <int D>
+__device__ __forceinline__ TileUnit tile_unit(const Kv4AttnArgs& a, const Kv4Request& r, int u) {
+    using L = TileLayout<D>;
+    TileUnit t;
+    t.e0 = u * L::ROWS;
+    t.rows = (int)min((long long)L::ROWS, r.qn * (long long)a.group - t.e0);
+    const int first = r.pos0 + t.e0 / a.group, last = r.pos0 + (t.e0 + t.rows - 1) / a.group;
+    const int hi = min(r.hi, last + 1);
+    t.lo = a.window > 0 ? max(0, min(first - a.window + 1, hi)) & ~(kKvGranule - 1) : 0;
+    t.n = hi > t.lo ? (hi - t.lo + L::NK - 1) / L::NK : 0;
+    return t;
+}
+
+// A request's blocks; 0 for the streaming kernel's requests.
+template <int D>
+__device__ __forceinline__ int tile_blocks(const Kv4AttnArgs& a, const Kv4Request& r) {
+    const long long pairs = r.qn * (long long)a.group;
+    return pairs <= a.max_cols ? 0 : (int)((pairs + TileLayout<D>::ROWS - 1) / TileLayout<D>::ROWS);
+}
+
+struct TileCursor {
+    Kv4Request r;
+    TileUnit t;
+    int b, h, u, blocks;
+    long long u0;
+};
+
+template <int D>
+__device__ __forceinline__ void tile_load(const Kv4AttnArgs& a, TileCursor& c) {
+    c.r = kv4_request(a, c.b);
+    c.blocks = tile_blocks<D>(a, c.r);
+    c.h = c.u = 0;
+    c.t.n = 0;
+    if (c.blocks) c.t = tile_unit<D>(a, c.r, 0);
+}
+
+// Moves the cursor forward to the unit that holds tile i of the list.
+template <int D>
+__device__ __forceinline__ void tile_seek(const Kv4AttnArgs& a, TileCursor& c, long long i) {
+    while (i >= c.u0 + c.t.n) {
+        c.u0 += c.t.n;
+        if (++c.u >= c.blocks) {
+            c.u = 0;
+            if (++c.h >= a.kv_heads || c.blocks == 0) {
+                c.b++;
+                tile_load<D>(a, c);
+                continue;
+            }
+        }
+        c.t = tile_unit<D>(a, c.r, c.u);
+    }
+}
+
+__device__ __forceinline__ void tc_mma_ts_f16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// N-major operand, 128-byte swizzle: 64-channel blocks `lead` bytes apart, 8-key groups 1024.
+__device__ __forceinline__ uint64_t smem_desc_sw128_n(uint32_t saddr, uint32_t lead) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+           (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+    uint32_t r[16];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) r[i] = __float_as_uint(v[h * 16 + i]);
+        tmem_st16(taddr + h * 16, r);
+    }
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Eight codes as F16 pairs (0 4, 1 5, 2 6, 3 7), times s2 plus m2.  A code under 1024's exponent is
+// 1024 + code (or 1024 + 16 code), made the code itself exactly before the one rounding.
+__device__ __forceinline__ uint4 widen8(uint32_t x, __half2 s2, __half2 m2) {
+    const __half2 k1024 = __half2half2(__ushort_as_half((unsigned short)0x6400));
+    const __half2 k16 = __half2half2(__ushort_as_half((unsigned short)0x2c00));  // 1/16
+    const __half2 k64 = __half2half2(__ushort_as_half((unsigned short)0xd400));  // -64
+    const uint32_t y = x >> 8;
+    const uint32_t w[4] = {(x & 0x000f000fu) | 0x64006400u, (x & 0x00f000f0u) | 0x64006400u,
+                           (y & 0x000f000fu) | 0x64006400u, (y & 0x00f000f0u) | 0x64006400u};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
+        const __half2 c = i & 1 ? __hfma2(h, k16, k64) : __hsub2(h, k1024);
+        const __half2 v = __hfma2(c, s2, m2);
+        o[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+__device__ __forceinline__ uint32_t dup_lo(uint32_t p) { return __byte_perm(p, p, 0x1010); }
+__device__ __forceinline__ uint32_t dup_hi(uint32_t p) { return __byte_perm(p, p, 0x3232); }
+__device__ __forceinline__ __half2 as_half2(uint32_t p) { return *reinterpret_cast<const __half2*>(&p); }
+
+// The channel of eight that sits at place p of a chunk.
+__host__ __device__ constexpr int chunk_channel(int p) { return (p >> 1) + 4 * (p & 1); }
+
+template <int D>
+__global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4AttnArgs a) {
+    using L = TileLayout<D>;
+    constexpr int G = L::G, MT = L::MT, NK = L::NK;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_slot;
+    __shared__ long long red[L::THREADS / 32];
+    __shared__ int pick_b, arrived;
+    __shared__ long long pick_u0;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + L::BAR);  // [deq warps][RING]
+    uint64_t* kfull = raw_full + kTlDeqWarps * L::RING;
+    uint64_t* kempty = kfull + L::KST;
+    uint64_t* vfull = kempty + L::KST;
+    uint64_t* vempty = vfull + L::VST;
+    uint64_t* sfull = vempty + L::VST;  // [2]: MT = 2 by row tile, MT = 1 by turn
+    uint64_t* pfull = sfull + 2;        // [2]
+    uint64_t* odone = pfull + 2;        // [2] (MT = 1: the first)
+    uint64_t* qfull = odone + 2;
+    if (tid == 0) {
+        for (int i = 0; i < kTlDeqWarps * L::RING; i++) mbar_init(&raw_full[i], 1);
+        for (int i = 0; i < L::KST; i++) mbar_init(&kfull[i], kTlDeqWarps), mbar_init(&kempty[i], 1);
+        for (int i = 0; i < L::VST; i++) mbar_init(&vfull[i], kTlDeqWarps), mbar_init(&vempty[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&sfull[i], 1), mbar_init(&pfull[i], 4), mbar_init(&odone[i], 1);
+        mbar_init(qfull, L::SM_WARPS);
+        fence_mbar_init();
+    }
+
+    // ---------------- the list's length; rows of blocks that see no key are zeroed here
+    const size_t head_row = (size_t)a.heads * D;
+    auto request_tiles = [&](int b, bool zero) {
+        const Kv4Request r = kv4_request(a, b);
+        const int blocks = tile_blocks<D>(a, r);
+        long long n = 0;
+        for (int u = 0; u < blocks; u++) {
+            const TileUnit t = tile_unit<D>(a, r, u);
+            n += t.n;
+            if (zero && t.n == 0 && (b + u) % (int)gridDim.x == (int)blockIdx.x)
+                for (int h = 0; h < a.kv_heads; h++)
+                    for (int e = t.e0; e < t.e0 + t.rows; e++) {
+                        uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + e / a.group) * head_row +
+                                                            (size_t)(h * a.group + e % a.group) * D);
+                        for (int i = 0; i < D / 8; i++) o[i] = make_uint4(0, 0, 0, 0);
+                    }
+        }
+        return n * a.kv_heads;
+    };
+    long long total = 0;
+    for (int b = tid; b < a.requests; b += L::THREADS) total += request_tiles(b, true);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
+    if (lane == 0) red[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < L::THREADS / 32; w++) total += red[w];
+    const long long ctas = min((long long)gridDim.x, total);
+    const int cta = blockIdx.x;
+    if (cta >= ctas) return;
+    const long long start = total * cta / ctas, end = total * (cta + 1) / ctas;
+    long long base = 0;
+    for (int b0 = 0; b0 < a.requests; b0 += L::THREADS) {
+        const int b = b0 + tid;
+        const long long n = b < a.requests ? request_tiles(b, false) : 0;
+        long long s = n;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, s, m);
+            if (lane >= m) s += x;
+        }
+        __syncthreads();
+        if (lane == 31) red[warp] = s;
+        __syncthreads();
+        long long all = 0;
+        for (int w = 0; w < L::THREADS / 32; w++) {
+            if (w < warp) s += red[w];
+            all += red[w];
+        }
+        if (n > 0 && start >= base + s - n && start < base + s) pick_b = b, pick_u0 = base + s - n;
+        base += all;
+        if (start < base) break;
+    }
+    if (warp == L::SM_WARPS + kTlDeqWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    TileCursor cur;
+    cur.b = pick_b;
+    cur.u0 = pick_u0;
+    tile_load<D>(a, cur);
+
+    if (warp < L::SM_WARPS) {
+        // ---------------- softmax: one thread a (row, head) pair of row tile `mt`
+        const int mt = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t o_tm = tmem + lanes + L::O_COL + mt * D;
+        uint32_t turns = 0;   // tiles this row tile has taken
+        uint32_t tiles = 0;   // tiles the CTA has taken (the value ring's turn)
+        bool ok = true;
+        for (long long pos = start; pos < end;) {
+            // both row tiles start a unit together: one that sits a unit out must not count for the next
+            asm volatile("bar.sync 2, %0;" ::"n"(L::SM_WARPS * 32) : "memory");
+            tile_seek<D>(a, cur, pos);
+            const Kv4Request r = cur.r;
+            const TileUnit un = cur.t;
+            const long long seg_end = min(end, cur.u0 + un.n);
+            const int j0 = (int)(pos - cur.u0), n = (int)(seg_end - pos);
+            const int e = mt * 128 + row;
+            const bool live = e < un.rows;                    // this thread has a pair
+            const bool tile_live = mt * 128 < un.rows;        // the row tile takes part
+            const int pair = un.e0 + (live ? e : 0);
+            const int qi = pair / a.group, head = cur.h * a.group + pair % a.group;
+            const int qpos = r.pos0 + qi;
+
+            // the query row: scaled by a power of two (largest entry to [2^13, 2^14)), F16, chunk order
+            const long long at = (r.q0 + qi) * a.qts + head * a.qhs;
+            float top = 0.0f;
+            auto load8q = [&](int c, float (&x)[8]) {
+                if (!live) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = 0.0f;
+                } else if (a.qvec) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at + c);
+                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const uint16_t h = (uint16_t)(ww[i >> 1] >> (16 * (i & 1)));
+                        x[i] = a.dt == 1 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = load_act(a.q, (size_t)(at + c + i), a.dt);
+                }
+            };
+#pragma unroll 4
+            for (int c = 0; c < D; c += 8) {
+                float x[8];
+                load8q(c, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+            }
+            int k2 = 0;
+            if (top > 0.0f && top < 3.0e38f) k2 = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -120), 120);
+            // a negative scale goes into the query's sign, so that c >= 0 below
+            const float up = copysignf(__uint_as_float((uint32_t)(k2 + 127) << 23), a.scale_log2);
+            const float c = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k2) << 23);
+#pragma unroll 4
+            for (int ch = 0; ch < D; ch += 8) {
+                float x[8];
+                load8q(ch, x);
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const __half2 h = __floats2half2_rn(x[i] * up, x[i + 4] * up);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                *reinterpret_cast<uint4*>(smem + L::Q + mt * L::Q_TILE + (ch >> 6) * 16384 + sw128_offset(row, ch & 63)) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qfull);
+
+            float mref = -1.0e30f, l = 0.0f;
+            uint32_t bad = 0;  // groups in which the row sees a NaN value
+            for (int j = 0; tile_live && j < n; j++, turns++) {
+                const int bi = MT == 2 ? mt : (int)(turns & 1);
+                const uint32_t par = MT == 2 ? turns & 1 : (turns >> 1) & 1;
+                const uint32_t s_tm = tmem + lanes + L::S_COL + bi * NK;
+                const int k0 = un.lo + (j0 + j) * NK;
+                if (ok) ok = mbar_wait(&sfull[bi], par, DEV_TIMEOUT_FULL);
+                tc_fence_after();
+                // every key of the tile seen by every pair of the block (pages outside the pool aside)?
+                const int first = r.pos0 + un.e0 / a.group, last = r.pos0 + (un.e0 + un.rows - 1) / a.group;
+                bool full = k0 + NK <= min(r.hi, first + 1) && (a.window == 0 || k0 > last - a.window);
+                uint32_t gone = 0;  // 16-key granules without a page
+                const int lowest = a.window > 0 ? qpos - a.window + 1 : 0, highest = min(r.hi - 1, qpos);
+                {
+                    const uint32_t vt = tiles + j;
+                    if (ok) ok = mbar_wait(&vfull[vt % L::VST], (vt / L::VST) & 1, DEV_TIMEOUT_FULL);
+                    const uint32_t* bm = reinterpret_cast<const uint32_t*>(smem + L::BAD + (vt % L::VST) * (G * (NK / 16) * 2));
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < G * (NK / 32); i++) any |= bm[i];
+                    if (any) {
+                        // bit 16 i + t of a group: key 16 i + t holds NaN; both a granule without a page
+                        // (every bit of every group) and NaN values come this way
+                        for (int i = 0; i < NK / 16; i++) {
+                            uint32_t all = 0xffffu;
+                            for (int gr = 0; gr < G; gr++) all &= reinterpret_cast<const uint16_t*>(bm)[gr * (NK / 16) + i];
+                            const int key = k0 + 16 * i;
+                            const int pg = key < r.hi ? a.table[cur.b * a.tstride + (key >> a.shift)] : -1;
+                            if (all == 0xffffu && (pg < 0 || pg >= a.pages)) {
+                                gone |= 1u << i;
+                                continue;
+                            }
+                            for (int gr = 0; gr < G; gr++) {
+                                const uint32_t m = reinterpret_cast<const uint16_t*>(bm)[gr * (NK / 16) + i];
+                                for (int t = 0; t < 16; t++)
+                                    if (((m >> t) & 1u) && key + t >= lowest && key + t <= highest) bad |= 1u << gr;
+                            }
+                        }
+                        full = full && gone == 0;
+                    }
+                }
+                auto masked = [&](int i) {  // key i of the tile
+                    const int key = k0 + i;
+                    return key < lowest || key > highest || ((gone >> (i >> 4)) & 1u);
+                };
+                float mx = -CUDART_INF_F;
+#pragma unroll 1
+                for (int q = 0; q < NK; q += 32) {
+                    float v[32];
+                    __syncwarp();
+                    tmem_ld32(s_tm + q, v);
+                    if (!full) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (masked(q + i)) v[i] = -CUDART_INF_F;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, v[i]);
+                }
+                mx = mx == -CUDART_INF_F ? mx : mx * c;
+                if (__any_sync(0xffffffffu, mx > mref + 15.0f)) {
+                    const float moved = fmaxf(mref, mx - 7.0f);
+                    const float f = ex2(mref - moved);
+                    mref = moved;
+                    l *= f;
+                    if (j > 0) {
+                        const uint32_t ot = turns - 1;  // the product of the tile before is in
+                        if (ok) ok = mbar_wait(&odone[MT == 2 ? mt : 0], ot & 1, DEV_TIMEOUT_FULL);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int q = 0; q < D; q += 32) {
+                            float v[32];
+                            tmem_ld32(o_tm + q, v);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) v[i] *= f;
+                            tmem_st32(o_tm + q, v);
+                        }
+                    }
+                }
+#pragma unroll 1
+                for (int q = 0; q < NK; q += 32) {
+                    float v[32];
+                    tmem_ld32(s_tm + q, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = ex2(fmaf(v[i], c, -mref));
+                    if (!full) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            if (masked(q + i)) v[i] = 0.0f;
+                    }
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        l += v[2 * i] + v[2 * i + 1];
+                        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    tmem_st16(s_tm + q / 2, w);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[bi]);
+            }
+            tiles += n;
+
+            // ---------------- the rows out, or this CTA's share of them into its slot
+            const bool whole = j0 == 0 && n == un.n;
+            float* slot = a.part + (size_t)(2 * cta + (pos == start ? 0 : 1)) * (L::ROWS * (D + 2));
+            if (tile_live) {
+                if (ok) ok = mbar_wait(&odone[MT == 2 ? mt : 0], (turns - 1) & 1, DEV_TIMEOUT_FULL);
+                tc_fence_after();
+                const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+#pragma unroll 1
+                for (int q = 0; q < D; q += 32) {
+                    float v[32];
+                    __syncwarp();
+                    tmem_ld32(o_tm + q, v);
+                    if (live) {
+                        const float by = (bad >> (q >> 6)) & 1u ? CUDART_NAN_F : inv;
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] *= by;
+#pragma unroll
+                        for (int w = 0; w < 32; w += 8) {
+                            float x[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) x[chunk_channel(i)] = v[w + i];
+                            if (whole) {
+                                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + qi) * head_row + (size_t)head * D + q + w) =
+                                    make_uint4(pack_act2(x[0], x[1], a.dt), pack_act2(x[2], x[3], a.dt),
+                                               pack_act2(x[4], x[5], a.dt), pack_act2(x[6], x[7], a.dt));
+                            } else {
+                                float4* dst = reinterpret_cast<float4*>(slot + e * D + q + w);
+                                __stcg(dst, make_float4(x[0], x[1], x[2], x[3]));
+                                __stcg(dst + 1, make_float4(x[4], x[5], x[6], x[7]));
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                tc_fence_before();  // the next unit's first product overwrites O after the next arrival
+                if (!whole && live)
+                    __stcg(reinterpret_cast<float2*>(slot + L::ROWS * D + 2 * e), make_float2(mref, l));
+            }
+            if (!whole) {
+                constexpr int NT = L::SM_WARPS * 32;
+                const int firstc = (int)(((cur.u0 + 1) * ctas - 1) / total);
+                const int lastc = (int)(((cur.u0 + un.n) * ctas - 1) / total);
+                __threadfence();
+                asm volatile("bar.sync 2, %0;" ::"n"(NT) : "memory");
+                if (tid == 0) arrived = atomicAdd(&a.count[firstc], 1);
+                asm volatile("bar.sync 2, %0;" ::"n"(NT) : "memory");
+                if (arrived == lastc - firstc) {
+                    __threadfence();
+                    if (tid == 0) a.count[firstc] = 0;
+                    auto slot_of = [&](int k) {
+                        return a.part + (size_t)(2 * k + (k == firstc && total * k / ctas != cur.u0 ? 1 : 0)) * (L::ROWS * (D + 2));
+                    };
+                    for (int i = tid; i < un.rows * (D / 4); i += NT) {
+                        const int ee = i / (D / 4), ch = (i % (D / 4)) * 4;
+                        float best = -1.0e30f;
+#pragma unroll 4
+                        for (int k = firstc; k <= lastc; k++) best = fmaxf(best, __ldcg(slot_of(k) + L::ROWS * D + 2 * ee));
+                        float ls = 0.0f;
+                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                        for (int k = firstc; k <= lastc; k++) {
+                            const float* sl = slot_of(k);
+                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(sl + L::ROWS * D + 2 * ee));
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(sl + ee * D + ch));
+                            const float f = ex2(ml.x - best);
+                            ls += f * ml.y;
+                            v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
+                        }
+                        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+                        const int p = un.e0 + ee;
+                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (r.q0 + p / a.group) * head_row +
+                                                  (size_t)(cur.h * a.group + p % a.group) * D + ch) =
+                            make_uint2(pack_act2(v.x * inv, v.y * inv, a.dt), pack_act2(v.z * inv, v.w * inv, a.dt));
+                    }
+                }
+            }
+            pos = seg_end;
+        }
+    } else if (warp < L::SM_WARPS + kTlDeqWarps) {
+        // ---------------- widening: warp w takes granules w GPW .. of every tile
+        const int w = warp - L::SM_WARPS;
+        uint8_t* ring = smem + L::RAW + w * L::RING * L::GB;
+        uint64_t* bar = raw_full + w * L::RING;
+        uint32_t tiles = 0, taken = 0;  // tiles widened, granules consumed
+        uint32_t there = 0;             // a bit a ring place: the granule was copied
+        bool ok = true;
+        for (long long pos = start; pos < end;) {
+            tile_seek<D>(a, cur, pos);
+            const Kv4Request r = cur.r;
+            const long long seg_end = min(end, cur.u0 + cur.t.n);
+            const int n = (int)(seg_end - pos);
+            const int lo = cur.t.lo + (int)(pos - cur.u0) * NK;
+            auto issue = [&](int q) {  // granule q of the warp's share of the segment, into place (taken + q) % RING
+                const int key = lo + (q / L::GPW) * NK + (w * L::GPW + q % L::GPW) * kKvGranule;
+                const int place = (int)((taken + q) % L::RING);
+                int page = -1;
+                if (key < r.hi) page = a.table[cur.b * a.tstride + (key >> a.shift)];
+                const bool got = page >= 0 && page < a.pages;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&bar[place], got ? L::GB : 0);
+                    if (got)
+                        bulk_g2s(ring + place * L::GB,
+                                 a.pool + kv4_granule<D>(page, a.kv_heads, cur.h, a.page_size, key & (a.page_size - 1)), L::GB,
+                                 &bar[place]);
+                }
+                there = (there & ~(1u << place)) | ((got ? 1u : 0u) << place);
+            };
+            for (int q = 0; q < L::RING && q < n * L::GPW; q++) issue(q);
+            for (int j = 0; j < n; j++, tiles++) {
+                const int kb = tiles % L::KST, vb = tiles % L::VST;
+                const int k0 = lo + j * NK + w * L::GPW * kKvGranule;  // the warp's first key
+                if (ok && tiles >= (uint32_t)L::KST) ok = mbar_wait(&kempty[kb], (tiles / L::KST - 1) & 1, DEV_TIMEOUT_EMPTY);
+                uint8_t* kt = smem + L::K + kb * L::KV_TILE;
+#pragma unroll
+                for (int gi = 0; gi < L::GPW; gi++) {
+                    const uint32_t q = taken + j * L::GPW + gi;
+                    const int place = (int)(q % L::RING);
+                    if (ok) ok = mbar_wait(&bar[place], (q / L::RING) & 1, DEV_TIMEOUT_FULL);
+                    const uint8_t* gran = ring + place * L::GB;
+                    const bool got = (there >> place) & 1u;
+                    const int t = lane & 3;
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const int tok = half * 8 + (lane >> 2);
+                        const bool seen = got && k0 + gi * kKvGranule + tok < r.hi;
+                        const int row = (w * L::GPW + gi) * kKvGranule + tok;
+                        uint32_t x[G][2];
+                        if constexpr (D == 64) {
+                            const uint2 u = *reinterpret_cast<const uint2*>(gran + kv4_key_word<D>(tok, 0, 2 * t));
+                            x[0][0] = u.x, x[0][1] = u.y;
+                        } else {
+#pragma unroll
+                            for (int gr = 0; gr < G; gr += 2) {
+                                const uint4 u = *reinterpret_cast<const uint4*>(gran + kv4_key_word<D>(tok, gr, 2 * t));
+                                x[gr][0] = u.x, x[gr][1] = u.y, x[gr + 1][0] = u.z, x[gr + 1][1] = u.w;
+                            }
+                        }
+#pragma unroll
+                        for (int gr = 0; gr < G; gr++) {
+                            const uint32_t p = seen ? *reinterpret_cast<const uint32_t*>(gran + kv4_kpar_off(D) + (tok * G + gr) * 4) : 0u;
+                            const __half2 s2 = as_half2(dup_lo(p)), m2 = as_half2(dup_hi(p));
+#pragma unroll
+                            for (int i = 0; i < 2; i++)
+                                *reinterpret_cast<uint4*>(kt + gr * L::SUB + sw128_offset(row, (2 * t + i) * 8)) = widen8(x[gr][i], s2, m2);
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kfull[kb]);
+
+                if (ok && tiles >= (uint32_t)L::VST) ok = mbar_wait(&vempty[vb], (tiles / L::VST - 1) & 1, DEV_TIMEOUT_EMPTY);
+                uint8_t* vt = smem + L::V + vb * L::KV_TILE;
+                uint16_t* bm = reinterpret_cast<uint16_t*>(smem + L::BAD) + vb * (G * (NK / 16));
+#pragma unroll
+                for (int gi = 0; gi < L::GPW; gi++) {
+                    const int place = (int)((taken + j * L::GPW + gi) % L::RING);
+                    const uint8_t* gran = ring + place * L::GB;
+                    const bool got = (there >> place) & 1u;
+                    const int kg = k0 + gi * kKvGranule;
+                    // NaN groups are widened to 0 (a key some row does not see must not reach it) and
+                    // named for the rows that do see them; so is a granule without a page
+#pragma unroll
+                    for (int gr = 0; gr < G; gr++) {
+                        const uint32_t p = *reinterpret_cast<const uint32_t*>(gran + kv4_vpar_off(D) + ((lane & 15) * G + gr) * 4);
+                        const bool nan = !got ? kg < r.hi : (kg + (lane & 15) < r.hi && ((p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u));
+                        const uint32_t m = __ballot_sync(0xffffffffu, nan) & 0xffffu;
+                        if (lane == 0) bm[gr * (NK / 16) + w * L::GPW + gi] = (uint16_t)m;
+                    }
+                    // lanes: piece pc of a row (D / 8 words in 8 pieces), four tokens at a time
+                    const int pc = lane & 7;
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; q4++) {
+                        const int tok = q4 * 4 + (lane >> 3);
+                        const bool seen = got && kg + tok < r.hi;
+                        const int row = (w * L::GPW + gi) * kKvGranule + tok;
+                        const uint8_t* src = gran + kv4_value_word<D>(tok, 0, pc);
+                        uint32_t x[G];
+                        if constexpr (D == 64) {
+                            x[0] = *reinterpret_cast<const uint32_t*>(src);
+                        } else if constexpr (D == 128) {
+                            const uint2 u = *reinterpret_cast<const uint2*>(src);
+                            x[0] = u.x, x[1] = u.y;
+                        } else {
+                            const uint4 u = *reinterpret_cast<const uint4*>(src);
+                            x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+                        }
+#pragma unroll
+                        for (int gr = 0; gr < G; gr++) {
+                            uint32_t p = seen ? *reinterpret_cast<const uint32_t*>(gran + kv4_vpar_off(D) + (tok * G + gr) * 4) : 0u;
+                            if ((p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u) p = 0u;
+                            *reinterpret_cast<uint4*>(vt + gr * L::SUB + sw128_offset(row, pc * 8)) =
+                                widen8(x[gr], as_half2(dup_lo(p)), as_half2(dup_hi(p)));
+                        }
+                    }
+                    __syncwarp();
+                    const int q = j * L::GPW + gi + L::RING;
+                    if (q < n * L::GPW) issue(q);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&vfull[vb]);
+            }
+            taken += n * L::GPW;
+            pos = seg_end;
+        }
+    } else if (lane == 0) {
+        // ---------------- the products
+        constexpr uint32_t id_s = idesc_f16_m128(NK);
+        constexpr uint32_t id_o = idesc_f16_m128(D) | (1u << 16);  // B is N-major
+        uint32_t tiles = 0, segs = 0;
+        uint32_t turn[2] = {0, 0};
+        bool ok = true;
+        auto scores = [&](int mt, int bi, uint32_t tile) {
+            const uint32_t q = smem_u32(smem + L::Q + mt * L::Q_TILE), k = smem_u32(smem + L::K + (tile % L::KST) * L::KV_TILE);
+            if (ok) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++)
+                    tc_mma_f16(tmem + L::S_COL + bi * NK, smem_desc_sw128(q + (kk >> 2) * 16384 + (kk & 3) * 32),
+                               smem_desc_sw128(k + (kk >> 2) * L::SUB + (kk & 3) * 32), id_s, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(&sfull[bi]);
+        };
+        auto values = [&](int mt, int bi, uint32_t tile, bool first) {
+            const uint32_t v = smem_u32(smem + L::V + (tile % L::VST) * L::KV_TILE);
+            if (ok) {
+#pragma unroll
+                for (int kk = 0; kk < NK / 16; kk++)
+                    tc_mma_ts_f16(tmem + L::O_COL + mt * D, tmem + L::S_COL + bi * NK + kk * 8,
+                                  smem_desc_sw128_n(v + kk * 2048, L::SUB), id_o, (!first || kk > 0) ? 1u : 0u);
+            }
+            tc_commit(&odone[MT == 2 ? mt : 0]);
+        };
+        for (long long pos = start; pos < end;) {
+            tile_seek<D>(a, cur, pos);
+            const long long seg_end = min(end, cur.u0 + cur.t.n);
+            const int n = (int)(seg_end - pos);
+            const int live = MT == 2 && cur.t.rows > 128 ? 2 : 1;
+            if (ok) ok = mbar_wait(qfull, segs & 1, DEV_TIMEOUT_FULL);
+            if (ok) ok = mbar_wait(&kfull[tiles % L::KST], (tiles / L::KST) & 1, DEV_TIMEOUT_FULL);
+            tc_fence_after();
+            for (int s = 0; s < live; s++) scores(s, MT == 2 ? s : (int)(turn[0] & 1), tiles);
+            tc_commit(&kempty[tiles % L::KST]);
+            for (int j = 0; j < n; j++, tiles++) {
+                const uint32_t nx = tiles + 1;
+                if (MT == 1 && j + 1 < n) {
+                    if (ok) ok = mbar_wait(&kfull[nx % L::KST], (nx / L::KST) & 1, DEV_TIMEOUT_FULL);
+                    tc_fence_after();
+                    scores(0, (int)((turn[0] + 1) & 1), nx);
+                    tc_commit(&kempty[nx % L::KST]);
+                }
+                if (ok) ok = mbar_wait(&vfull[tiles % L::VST], (tiles / L::VST) & 1, DEV_TIMEOUT_FULL);
+                for (int s = 0; s < live; s++) {
+                    const int bi = MT == 2 ? s : (int)(turn[0] & 1);
+                    if (ok) ok = mbar_wait(&pfull[bi], MT == 2 ? turn[s] & 1 : (turn[0] >> 1) & 1, DEV_TIMEOUT_FULL);
+                    tc_fence_after();
+                    values(s, bi, tiles, j == 0);
+                    if (MT == 2 && j + 1 < n) {
+                        if (s == 0) {
+                            if (ok) ok = mbar_wait(&kfull[nx % L::KST], (nx / L::KST) & 1, DEV_TIMEOUT_FULL);
+                            tc_fence_after();
+                        }
+                        scores(s, s, nx);
+                    }
+                    turn[s]++;
+                }
+                tc_commit(&vempty[tiles % L::VST]);
+                if (MT == 2 && j + 1 < n) tc_commit(&kempty[nx % L::KST]);
+            }
+            segs++;
+            pos = seg_end;
+        }
+        // the last commit of all: nothing of this CTA's is in flight when it frees its tensor memory
+        if (ok) mbar_wait(&vempty[(tiles - 1) % L::VST], ((tiles - 1) / L::VST) & 1, DEV_TIMEOUT_EMPTY);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == L::SM_WARPS + kTlDeqWarps) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    }
+}
+
+namespace {
+
+template <int D>
+cudaError_t tile_launch(const Kv4AttnArgs& a, cudaStream_t stream) {
+    using L = TileLayout<D>;
+    auto kern = kv4_tile_kernel<D>;
+    cudaError_t e = func_attrs(reinterpret_cast<const void*>(kern), L::ALLOC, false);
+    if (e != cudaSuccess) return e;
+    kern<<<sm_count(), L::THREADS, L::ALLOC, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t kv4_tile_part_floats(int D) { return (size_t)(D == 256 ? 128 : 256) * (D + 2); }
+
+cudaError_t kv4_tile_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream) {
+    if (D == 64) return tile_launch<64>(a, stream);
+    if (D == 128) return tile_launch<128>(a, stream);
+    return tile_launch<256>(a, stream);
+}
+
+}  // namespace sx

@@ -12,7 +12,7 @@ def held(x):
     """(held values f64, steps f64, distance of (x - m)/s from the nearest tie) of x [T, H, D]: the
     group's parameters by the format's f32 formula, the codes by a division in 64 bits."""
     t, h, d = x.shape
-    y32 = x.float().clamp(-65504.0, 65504.0).reshape(t, h, d // GROUP, GROUP)
+    y32 = x.float().clamp(-57344.0, 57344.0).reshape(t, h, d // GROUP, GROUP)
     lo, hi = y32.amin(-1, keepdim=True), y32.amax(-1, keepdim=True)
     step = ((hi - lo) * np.float32(1.0 / 15.0).item()).half().double()
     low = lo.half().double()

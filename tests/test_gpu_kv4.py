@@ -142,7 +142,7 @@ def test_write_of_extreme_values():
     x[0, 0, 3] = math.inf
     x[1, 0, 70] = -math.inf
     x[2, 0, 5] = math.nan
-    x[3, 0, 0], x[3, 0, 1] = 3e38, -3e38  # finite, past f16: held as its largest
+    x[3, 0, 0], x[3, 0, 1] = 3e38, -3e38  # finite, past the format's largest
     x[4, 0, :] = 65504.0
     x = x.to(torch.bfloat16)
     c = sx().Kv4Cache(1, 1, 128, 16)
@@ -332,6 +332,35 @@ def test_nan_and_infinity_reach_only_the_rows_that_see_them(n):
     assert torch.isnan(got[first:n, 4:]).all()
     assert torch.equal(got[:first], clean[:first]) and torch.equal(got[:n, :4], clean[:n, :4])
     assert torch.equal(got[n:], clean[n:])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 3, 130])
+def test_nan_values_reach_only_the_rows_that_see_them(d, n):
+    st = Step(24, d, torch.bfloat16, 4, 2, 16, [(300, n), (60, 1)])
+    clean = st.run()
+    at = 299 if n == 3 else 290
+    v = st.v[at:at + 1].clone()
+    v[0, 1, d - 3] = math.nan
+    sx().kv4_write(st.cache, st.k[at:at + 1], v, st.slots[at:at + 1])
+    got = st.run()
+    first = max(0, at - (300 - n))
+    group = slice(d - 64, d)  # the channels of the NaN's group, in the heads of key head 1
+    assert torch.isnan(got[first:n, 2:, group]).all()
+    assert torch.equal(got[:first], clean[:first]) and torch.equal(got[:n, :2], clean[:n, :2])
+    assert torch.equal(got[:n, :, :d - 64], clean[:n, :, :d - 64])
+    assert torch.equal(got[n:], clean[n:])
+
+
+def test_values_of_any_magnitude():
+    """Steps far below and above 1, and growing along the keys (the streaming kernel's reference follows them)."""
+    for scale in (1e-3, 1.0, 2000.0):
+        for n in (1, 40):
+            st = Step(25, 128, torch.bfloat16, 8, 2, 16, [(500, n)])
+            ramp = torch.logspace(-2, 1, 500, device="cuda")[:, None, None] * scale
+            st.v = (st.v.float() * ramp).to(torch.bfloat16)
+            sx().kv4_write(st.cache, st.k, st.v, st.slots)
+            st.check(st.run())
 
 
 def test_attention_past_32_bit_offsets():
