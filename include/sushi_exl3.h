@@ -379,9 +379,10 @@ sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slot
  * Positions whose page id is outside the pool, or past table_width pages, count as unseen.
  * q [tokens][heads][head_dim] with strides in elements, channels contiguous; out contiguous and
  * 16-byte aligned; both of `dtype`, BF16 or F16 (SX_ERR_BAD_DTYPE for F32: the products take 16-bit operands).  heads is a
- * multiple of kv_heads; scale finite.  workspace: sx_kv4_attention_workspace_bytes(...) bytes,
- * 16-byte aligned, ZEROED before its first use; every call leaves what has to be zero at zero, also
- * for calls of other sizes.  Calls that may run at the same time need their own. */
+ * multiple of kv_heads; scale finite; requests * kv_heads * table_width * page_size / 16 below 2^31
+ * (and as many tiles of keys times blocks of rows, where rows are many), else SX_ERR_BAD_SHAPE.
+ * workspace: sx_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned; it keeps nothing between
+ * calls, but calls that may run at the same time need their own. */
 size_t sx_kv4_attention_workspace_bytes(const sx_kv4* cache, int32_t requests, int32_t tokens, int32_t heads,
                                         int32_t max_q);
 sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q, int64_t q_token_stride,

@@ -2,7 +2,7 @@
 // device: at most max_cols (row, query head) pairs a key head go to the streaming kernel, whose MMAs
 // carry 8 or 16 columns, the rest to the tile kernel, whose carry 128 rows.
 #include <cuda_runtime.h>
-#include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "sx_kv4_attn.cuh"
@@ -18,13 +18,10 @@ int stream_cols(const sx_kv4* c, int heads, int max_q) {
     return heads / c->kv_heads > 8 || (most > 8 && most <= 16) ? 16 : 8;
 }
 
-// The workspace: a counter a CTA, then two partial slots a CTA, of 16 columns (streaming kernel) or of
-// a block of rows (tile kernel, which runs after it on the stream and takes the same space).
-size_t counters_bytes() { return ((size_t)kv4_max_ctas() * sizeof(int) + 15) / 16 * 16; }
-size_t part_bytes(int D, bool tile) {
-    const size_t stream = (size_t)kv4_max_ctas() * 2 * 16 * (D + 2) * sizeof(float);
-    return std::max(stream, tile ? (size_t)sm_count() * 2 * kv4_tile_part_floats(D) * sizeof(float) : 0);
-}
+// The workspace: the two partial slots of every CTA, the streaming kernel's (16 columns), then the
+// tile kernel's (a block of rows) where the call can reach it.  Nothing in it outlives the call.
+size_t stream_bytes(int D, int cols) { return (size_t)kv4_stream_grid(D, cols) * 2 * kStRows * (D + 2) * sizeof(float); }
+size_t tile_bytes(int D) { return (size_t)sm_count() * 2 * kv4_tile_rows(D) * (D + 2) * sizeof(float); }
 
 }  // namespace
 
@@ -34,8 +31,8 @@ size_t sx_kv4_attention_workspace_bytes(const sx_kv4* cache, int32_t requests, i
                                         int32_t max_q) {
     (void)requests, (void)tokens;
     if (!cache || !kv4_dim_ok(cache->head_dim) || cache->kv_heads < 1 || heads < cache->kv_heads || max_q < 1) return 0;
-    return counters_bytes() +
-           part_bytes(cache->head_dim, most_pairs(cache, heads, max_q) > stream_cols(cache, heads, max_q));
+    const int D = cache->head_dim, cols = stream_cols(cache, heads, max_q);
+    return stream_bytes(D, cols) + (most_pairs(cache, heads, max_q) > cols ? tile_bytes(D) : 0);
 }
 
 sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q, int64_t q_token_stride,
@@ -48,6 +45,14 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     if (dtype != SX_DT_F16 && dtype != SX_DT_BF16) return SX_ERR_BAD_DTYPE;
     if (tokens < 0 || heads < 1 || heads % cache->kv_heads || requests < 1 || table_width < 1 ||
         table_stride < table_width || max_q < 1 || window < 0 || !std::isfinite(scale))
+        return SX_ERR_BAD_SHAPE;
+    // the work lists count steps (of 16 tokens at the smallest; tiles of keys) in 32 bits
+    if ((long long)requests * cache->kv_heads * ((long long)table_width * (cache->page_size / kKvGranule)) > INT_MAX)
+        return SX_ERR_BAD_SHAPE;
+    const long long blocks = (long long)tokens * (heads / cache->kv_heads) / kv4_tile_rows(cache->head_dim) + requests;
+    const long long tiles = (long long)table_width * cache->page_size / kv4_tile_keys(cache->head_dim) + 1;
+    if (most_pairs(cache, heads, max_q) > stream_cols(cache, heads, max_q) &&
+        (double)blocks * (double)tiles * cache->kv_heads > INT_MAX)
         return SX_ERR_BAD_SHAPE;
     if (tokens == 0) return SX_OK;
     if (!q || !cu_q || !kv_lens || !table || !out || !workspace) return SX_ERR_NULL_POINTER;
@@ -66,13 +71,18 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     a.qvec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     a.scale_log2 = (float)(scale * 1.4426950408889634), a.window = window;
     a.max_cols = stream_cols(cache, heads, max_q);
-    a.count = static_cast<int*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + counters_bytes());
+    a.part = static_cast<float*>(workspace);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = kv4_stream_launch(a, cache->head_dim, s);
+    const int D = cache->head_dim;
+    cudaError_t e = kv4_stream_launch(a, D, s);
     if (e != cudaSuccess) return cuda_status(e, "kv4_attention stream launch");
-    if (most_pairs(cache, heads, max_q) <= a.max_cols) return SX_OK;
-    return cuda_status(kv4_tile_launch(a, cache->head_dim, s), "kv4_attention tile launch");
+    if (most_pairs(cache, heads, max_q) <= a.max_cols)
+        return cuda_status(kv4_join_launch(a, nullptr, D, s), "kv4_attention join launch");
+    Kv4AttnArgs t = a;
+    t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_bytes(D, a.max_cols));
+    e = kv4_tile_launch(t, D, s);
+    if (e != cudaSuccess) return cuda_status(e, "kv4_attention tile launch");
+    return cuda_status(kv4_join_launch(a, &t, D, s), "kv4_attention join launch");
 }
 
 }  // extern "C"

@@ -22,8 +22,7 @@ struct Kv4AttnArgs {
     float scale_log2;  // scale * log2(e)
     int window;
     int max_cols;      // requests of at most this many (row, head) pairs a key head are the streaming kernel's
-    float* part;       // partial sums of units that several CTAs share
-    int* count;        // arrivals, zero between calls
+    float* part;       // the kernel's partial slots, two a CTA (units that several CTAs share)
 };
 
 // One request of a call: its rows, and the positions its keys occupy.
@@ -60,11 +59,130 @@ __device__ __forceinline__ uint32_t pack_act2(float a, float b, int dt) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The streaming kernel (sx_kv4_stream.cu).  kv4_max_ctas: CTAs no launch of it passes.
-inline int kv4_max_ctas() { return 4 * sm_count(); }
+// ------------------------------------------------------------------ the work lists
+// Both kernels lay their units' steps end to end and cut the list into equal runs, one a CTA: run c is
+// steps [start(c), start(c + 1)).
+struct RunCut {
+    int ctas, per, rem;  // the first rem runs have per + 1 steps
+    __device__ __forceinline__ RunCut(int total, int most) {
+        ctas = max(1, min(most, total));
+        per = (int)((unsigned)total / (unsigned)ctas);
+        rem = total - per * ctas;
+    }
+    __device__ __forceinline__ int start(int c) const { return c * per + min(c, rem); }
+    __device__ __forceinline__ int owner(int step) const {
+        const int head = rem * (per + 1);
+        return step < head ? step / (per + 1) : rem + (step - head) / per;
+    }
+};
+
+// Streaming kernel: a step is 256/D granules of one unit = (request, key head).
+constexpr int kStWarps = 4;
+constexpr int kStRows = 16;  // columns of a partial slot
+template <int D>
+__device__ __forceinline__ int stream_steps(const Kv4AttnArgs& a, const Kv4Request& r) {
+    constexpr int T = kKvGranule * (256 / D);
+    if (r.qn * (long long)a.group > a.max_cols) return 0;
+    return (r.hi - r.lo + T - 1) / T;
+}
+// Every warp of a CTA that runs has a step to take.
+__device__ __forceinline__ int stream_most(int total, int grid) { return min(grid, (total + kStWarps - 1) / kStWarps); }
+
+// Tile kernel: a step is a tile of kv4_tile_keys(D) keys of one unit = (request, key head, block of
+// kv4_tile_rows(D) (row, query head) pairs).
+__host__ __device__ constexpr int kv4_tile_rows(int D) { return D == 256 ? 128 : 256; }
+__host__ __device__ constexpr int kv4_tile_keys(int D) { return D == 256 ? 64 : 128; }
+
+struct TileUnit {
+    int e0, rows;  // pairs [e0, e0 + rows)
+    int lo, n;     // n tiles of keys from position lo
+};
+
+template <int D>
+__device__ __forceinline__ TileUnit tile_unit(const Kv4AttnArgs& a, const Kv4Request& r, int u) {
+    TileUnit t;
+    t.e0 = u * kv4_tile_rows(D);
+    t.rows = (int)min((long long)kv4_tile_rows(D), r.qn * (long long)a.group - t.e0);
+    const int first = r.pos0 + t.e0 / a.group, last = r.pos0 + (t.e0 + t.rows - 1) / a.group;
+    const int hi = min(r.hi, last + 1);
+    t.lo = a.window > 0 ? max(0, min(first - a.window + 1, hi)) & ~(kKvGranule - 1) : 0;
+    t.n = hi > t.lo ? (hi - t.lo + kv4_tile_keys(D) - 1) / kv4_tile_keys(D) : 0;
+    return t;
+}
+
+// A request's blocks; 0 for the streaming kernel's requests.
+template <int D>
+__device__ __forceinline__ int tile_blocks(const Kv4AttnArgs& a, const Kv4Request& r) {
+    const long long pairs = r.qn * (long long)a.group;
+    return pairs <= a.max_cols ? 0 : (int)((pairs + kv4_tile_rows(D) - 1) / kv4_tile_rows(D));
+}
+
+// Sum of v over the block's W warps, and the running sum before this thread (both in thread order).
+template <int W>
+__device__ __forceinline__ int block_scan(int v, int* red, int& before) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int s = v;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, s, m);
+        if (lane >= m) s += x;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = s;
+    __syncthreads();
+    int all = 0;
+    before = s - v;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        if (w < warp) before += red[w];
+        all += red[w];
+    }
+    return all;
+}
+
+// The list's length by steps(b) of every request, W warps together; n0 is steps(threadIdx.x).
+template <int W, typename F>
+__device__ __forceinline__ int list_total(int requests, int* red, int& n0, F steps) {
+    n0 = (int)threadIdx.x < requests ? steps((int)threadIdx.x) : 0;
+    int v = n0;
+    for (int b = threadIdx.x + W * 32; b < requests; b += W * 32) v += steps(b);
+    v = __reduce_add_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) all += red[w];
+    return all;
+}
+
+// The request that holds step `at` of the list, and the list position of its first step (in `pick`).
+template <int W, typename F>
+__device__ __forceinline__ void list_find(int requests, int* red, int* pick, int n0, int at, F steps) {
+    int base = 0;
+    for (int b0 = 0; b0 < requests; b0 += W * 32) {
+        const int b = b0 + threadIdx.x;
+        const int n = b0 == 0 ? n0 : (b < requests ? steps(b) : 0);
+        int before;
+        const int all = block_scan<W>(n, red, before);
+        before += base;
+        if (n > 0 && at >= before && at < before + n) pick[0] = b, pick[1] = before;
+        base += all;
+        if (at < base) break;
+    }
+    __syncthreads();
+}
+
+// Programmatic dependent launch: the next kernel of the call may start; this one's predecessors done.
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The streaming kernel (sx_kv4_stream.cu); its grid.
+int kv4_stream_grid(int D, int max_cols);
 cudaError_t kv4_stream_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream);
-// The tile kernel (sx_kv4_tile.cu), one CTA an SM; floats of one of its two partial slots a CTA.
-size_t kv4_tile_part_floats(int D);
+// The tile kernel (sx_kv4_tile.cu): one CTA an SM.
 cudaError_t kv4_tile_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream);
+// The join of the units that several CTAs of either kernel shared (sx_kv4_join.cu): `tile` null
+// where that kernel did not run.
+cudaError_t kv4_join_launch(const Kv4AttnArgs& stream_args, const Kv4AttnArgs* tile, int D, cudaStream_t stream);
 
 }  // namespace sx

@@ -15,18 +15,17 @@
 //
 // Work: the units' steps (4.5 KB of one head: 256/D granules of 16 tokens) laid end to end and cut
 // into equal runs, one a CTA, so ragged lengths balance; a CTA's warps take its steps in turn, each
-// with its own ring of bulk copies.  A unit that several CTAs share is joined by the last of them to
-// arrive, in CTA order (a counter, no CTA waits), so results do not depend on the arrival order.
+// with its own ring of bulk copies.  A unit that several CTAs share is joined by sx_kv4_join.cu.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "sx_kv4_attn.cuh"
 
 namespace sx {
 
-constexpr int kStWarps = 4;
 constexpr int kStThreads = kStWarps * 32;
 constexpr int kStStages = 3;
 
@@ -48,26 +47,19 @@ struct StreamLayout {
     static constexpr int TOTAL = BAR + kStWarps * kStStages * 8;
 };
 
-// A walk over the units' steps: request b, key head h, steps [u0, u0 + n) of the whole list.
+// A walk over the units' steps: request b, key head h; the unit's n steps begin at step `beg` of this
+// CTA's run (negative where the unit began in an earlier CTA's).
 struct StreamCursor {
     Kv4Request r;
-    int b, h, n;
-    long long u0;
+    int b, h, n, beg;
 };
 
+// Moves the cursor forward to the unit that holds step i of the run.
 template <int D>
-__device__ __forceinline__ int stream_steps(const Kv4AttnArgs& a, const Kv4Request& r) {
-    constexpr int T = kKvGranule * (256 / D);
-    if (r.qn * (long long)a.group > a.max_cols) return 0;
-    return (r.hi - r.lo + T - 1) / T;
-}
-
-// Moves the cursor forward to the unit that holds step i of the list.
-template <int D>
-__device__ __forceinline__ void stream_seek(const Kv4AttnArgs& a, StreamCursor& c, long long i) {
-    while (i >= c.u0 + c.n) {
-        c.u0 += c.n;
-        if (++c.h == a.kv_heads || c.n == 0) {
+__device__ __forceinline__ void stream_seek(const Kv4AttnArgs& a, StreamCursor& c, int i) {
+    while (i >= c.beg + c.n) {
+        c.beg += c.n;
+        if (++c.h >= a.kv_heads || c.n == 0) {
             c.h = 0;
             c.b++;
             c.r = kv4_request(a, c.b);
@@ -86,14 +78,34 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // four are tokens t and 4 + (t ^ 1), which the block's word order spreads over the banks).
 __device__ __forceinline__ int row_token(int r) { return (r & 8) + ((r & 1) ? 4 + (((r & 7) >> 1) ^ 1) : ((r & 7) >> 1)); }
 
+// A token's parameters (step, minimum) of every group.
+template <int G>
+__device__ __forceinline__ void load_params(const uint8_t* p, float2 (&f)[G]) {
+    uint32_t w[G];
+    if constexpr (G == 1) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (G == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    }
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) f[gr] = __half22float2(*reinterpret_cast<const __half2*>(&w[gr]));
+}
+
 template <int D, int NT>
-__global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_stream_kernel(Kv4AttnArgs a) {
+__host__ __device__ constexpr int stream_resident() {
+    return NT == 1 && D <= 128 ? 3 : 2;
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stream_kernel(Kv4AttnArgs a) {
     using L = StreamLayout<D, NT>;
     constexpr int G = L::G, GS = L::GS, COLS = L::COLS;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long red[kStWarps];
-    __shared__ int pick_b, arrived;
-    __shared__ long long pick_u0;
+    __shared__ int red[kStWarps], pick[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::BAR) + warp * kStStages;
@@ -103,82 +115,47 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
     fence_mbar_init();
 
     // ---------------- the list: its length, then the unit of this CTA's first step
-    long long total = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += kStThreads) {
-        const int b = b0 + tid;
-        total += b < a.requests ? (long long)stream_steps<D>(a, kv4_request(a, b)) * a.kv_heads : 0;
-    }
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
-    if (lane == 0) red[warp] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kStWarps; w++) total += red[w];
-    // every warp of a CTA that runs has a step to take
-    const long long ctas = min((long long)gridDim.x, (total + kStWarps - 1) / kStWarps);
+    pdl_release();
     const int cta = blockIdx.x;
-
-    // Rows that no unit writes: requests without a visible position, rows past the last request.
-    const size_t row_units = (size_t)a.heads * D / 8;
-    for (int b = cta; b <= a.requests; b += gridDim.x) {
-        int r0, rn;
-        if (b < a.requests) {
-            const Kv4Request r = kv4_request(a, b);
-            r0 = r.q0;
-            rn = r.hi <= r.lo && r.qn * (long long)a.group <= a.max_cols ? r.qn : 0;
-        } else {
-            r0 = min(max(a.cu_q[a.requests], 0), a.tokens);
-            rn = a.tokens - r0;
+    const int past = min(max(a.cu_q[a.requests], 0), a.tokens);  // rows from here on belong to no request
+    auto steps = [&](int b) {
+        const Kv4Request r = kv4_request(a, b);
+        const int n = stream_steps<D>(a, r);
+        if (n == 0 && r.qn > 0 && r.hi <= r.lo && r.qn * (long long)a.group <= a.max_cols && b % (int)gridDim.x == cta) {
+            // no key to see: no unit writes these rows
+            uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)r.q0 * a.heads * D);
+            for (size_t i = 0; i < (size_t)r.qn * a.heads * D / 8; i++) o[i] = make_uint4(0, 0, 0, 0);
         }
-        uint4* o = reinterpret_cast<uint4*>(a.out) + r0 * row_units;
-        for (size_t i = tid; i < rn * row_units; i += kStThreads) o[i] = make_uint4(0, 0, 0, 0);
+        return n * a.kv_heads;
+    };
+    int n0;
+    const int total = list_total<kStWarps>(a.requests, red, n0, steps);
+    const RunCut run(total, stream_most(total, gridDim.x));
+    if (past < a.tokens) {
+        uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)past * a.heads * D);
+        const size_t n = (size_t)(a.tokens - past) * a.heads * D / 8;
+        for (size_t i = (size_t)cta * kStThreads + tid; i < n; i += (size_t)gridDim.x * kStThreads) o[i] = make_uint4(0, 0, 0, 0);
     }
-    if (cta >= ctas) return;
-    const long long start = total * cta / ctas, end = total * (cta + 1) / ctas;
-
-    long long base = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += kStThreads) {
-        const int b = b0 + tid;
-        const long long n = b < a.requests ? (long long)stream_steps<D>(a, kv4_request(a, b)) * a.kv_heads : 0;
-        long long s = n;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, s, m);
-            if (lane >= m) s += x;
-        }
-        __syncthreads();
-        if (lane == 31) red[warp] = s;
-        __syncthreads();
-        long long all = 0;
-#pragma unroll
-        for (int w = 0; w < kStWarps; w++) {
-            if (w < warp) s += red[w];
-            all += red[w];
-        }
-        if (n > 0 && start >= base + s - n && start < base + s) {
-            pick_b = b;
-            pick_u0 = base + s - n;
-        }
-        base += all;
-        if (start < base) break;
-    }
-    __syncthreads();
+    if (total == 0 || cta >= run.ctas) return;
+    const int start = run.start(cta);
+    const int len = run.start(cta + 1) - start;  // this CTA's run
+    list_find<kStWarps>(a.requests, red, pick, n0, start, steps);
     StreamCursor cur;
-    cur.b = pick_b;
+    cur.b = pick[0];
     cur.r = kv4_request(a, cur.b);
     cur.n = stream_steps<D>(a, cur.r);
-    cur.h = (int)((start - pick_u0) / cur.n);
-    cur.u0 = pick_u0 + (long long)cur.h * cur.n;
+    const int into = start - pick[1];
+    cur.h = into / cur.n;
+    cur.beg = cur.h * cur.n - into;
     StreamCursor ahead = cur;
 
-    // ---------------- this warp's ring: step start + warp + 4 k in stage k % S
+    // ---------------- this warp's ring: step warp + 4 k of the run in stage k % S
     uint32_t valid = 0;  // 4 bits a stage: the granules that were copied
-    long long next = start + warp;
+    int next = warp;
     auto issue = [&](int st) {
-        if (next < end) {
+        if (next < len) {
             stream_seek<D>(a, ahead, next);
-            const int pos = ahead.r.lo + ((int)(next - ahead.u0) * GS + (lane < GS ? lane : 0)) * kKvGranule;
+            const int pos = ahead.r.lo + ((next - ahead.beg) * GS + (lane < GS ? lane : 0)) * kKvGranule;
             int page = -1;
             if (lane < GS && pos < ahead.r.hi) page = a.table[ahead.b * a.tstride + (pos >> a.shift)];
             const bool ok = page >= 0 && page < a.pages;
@@ -202,28 +179,30 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
     float* l_sm = m_sm + kStWarps * COLS;
     float* merge = reinterpret_cast<float*>(smem + L::MERGE);
     const int tok0 = row_token(g);                   // fragment row g; row g + 8 is token tok0 + 8
+    const uint8_t* q_lane = smem + L::Q + (g * D + 2 * t * 8) * 2;
     const int vt[4] = {t, 4 + (t ^ 1), 8 + t, 12 + (t ^ 1)};  // rows 2t, 2t+1, 2t+8, 2t+9
 
-    long long mine = start + warp;  // this warp's next step
+    int mine = warp;  // this warp's next step of the run
     int stage = 0;
     uint32_t parity = 0;
     bool alive = true;
-    for (long long pos = start; pos < end;) {
+    for (int pos = 0; pos < len;) {
         stream_seek<D>(a, cur, pos);
-        const long long seg_end = min(end, cur.u0 + cur.n);
+        const int seg_end = min(len, cur.beg + cur.n);
         const Kv4Request r = cur.r;
         const int ncols = r.qn * a.group;
 
         // ---------------- the unit's query columns: power-of-two scale, F16, fragment order
         __syncthreads();
-        for (int c = warp; c < COLS; c += kStWarps) {
-            constexpr int E = D / 32;
-            float x[E];
-            const int qi = c / a.group, hh = cur.h * a.group + c % a.group;
-            float top = 0.0f;
+        constexpr int E = D / 32, CW = COLS / kStWarps;  // entries a lane, columns a warp
+        float x[CW][E];
 #pragma unroll
-            for (int e = 0; e < E; e++) x[e] = 0.0f;
+        for (int w = 0; w < CW; w++) {
+            const int c = warp + w * kStWarps;
+#pragma unroll
+            for (int e = 0; e < E; e++) x[w][e] = 0.0f;
             if (c < ncols) {
+                const int qi = c / a.group, hh = cur.h * a.group + c - qi * a.group;
                 const long long at = (r.q0 + qi) * a.qts + hh * a.qhs + lane * E;
                 if (a.qvec && E >= 4) {
 #pragma unroll
@@ -231,17 +210,21 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
                         float v4[4];
                         load_act4(a.q, (size_t)(at + e), a.dt, v4);
 #pragma unroll
-                        for (int j = 0; j < 4 && e + j < E; j++) x[e + j] = v4[j];
+                        for (int j = 0; j < 4 && e + j < E; j++) x[w][e + j] = v4[j];
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < E; e++) x[e] = load_act(a.q, (size_t)(at + e), a.dt);
+                    for (int e = 0; e < E; e++) x[w][e] = load_act(a.q, (size_t)(at + e), a.dt);
                 }
             }
+        }
 #pragma unroll
-            for (int e = 0; e < E; e++) top = fmaxf(top, fabsf(x[e]));
+        for (int w = 0; w < CW; w++) {
+            const int c = warp + w * kStWarps;
+            float top = 0.0f;
 #pragma unroll
-            for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+            for (int e = 0; e < E; e++) top = fmaxf(top, fabsf(x[w][e]));
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // entries of no sign order as integers
             // 2^k with top * 2^k in [2^13, 2^14); 1 for a column of zeros or without a finite maximum
             int k = 0;
             if (top > 0.0f && top < 3.0e38f) k = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -120), 120);
@@ -251,7 +234,7 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
             for (int e = 0; e < E; e++) {
                 const int ch = lane * E + e, n = ch & 7;
                 const bool odd = n & 1;
-                const __half hq = __float2half_rn(odd ? x[e] * up * 0.0625f : x[e] * up);
+                const __half hq = __float2half_rn(odd ? x[w][e] * up * 0.0625f : x[w][e] * up);
                 sum += odd ? __half2float(hq) * 16.0f : __half2float(hq);
                 // fragment order of a word: nibbles 0 4 2 6 1 5 3 7
                 const int place = ((n & 1) << 2) | (n & 2) | (n >> 2);
@@ -278,14 +261,14 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
             }
 
         // ---------------- this warp's steps of the segment
-        float o[G][4][NT][4], mn[G][NT][2], l[NT][2], mref[NT][2];
-        float se = -26.0f, sthr = 0.0f;  // steps seen so far are at most sthr = 2^se
+        float o[G][4][NT][4], mn[G][NT][2], l[NT][2], mref[NT][2], thr[NT][2];
+        float sthr = 0.0f, lim = 41.0f;  // steps so far are at most sthr; a score may pass its reference by lim
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 l[nt][j] = 0.0f;
-                mref[nt][j] = -1.0e30f;
+                mref[nt][j] = thr[nt][j] = -1.0e30f;
 #pragma unroll
                 for (int gr = 0; gr < G; gr++) mn[gr][nt][j] = 0.0f;
             }
@@ -298,17 +281,13 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
 #pragma unroll
                     for (int j = 0; j < 4; j++) o[gr][mt][nt][j] = 0.0f;
 
-        for (; mine < seg_end; mine += kStWarps) {
-            if (alive) alive = mbar_wait(&bar[stage], parity, DEV_TIMEOUT_FULL);
-            const uint8_t* st = ring + stage * L::STEP;
-            const int p0 = r.lo + (int)(mine - cur.u0) * GS * kKvGranule;
-            const uint32_t vm = (valid >> (4 * stage)) & 15u;
-            // every key of the step seen by every row?
-            const bool full = vm == (1u << GS) - 1 && p0 + GS * kKvGranule <= min(r.hi, r.pos0 + 1) &&
-                              (a.window == 0 || p0 > r.pos0 + r.qn - 1 - a.window);
-
+        // steps at positions [full_lo, full_hi) are seen whole by every row
+        const int full_hi = min(r.hi, r.pos0 + 1) - GS * kKvGranule;
+        const int full_lo = a.window > 0 ? r.pos0 + r.qn - a.window : 0;
+        auto step = [&](const uint8_t* st, int p0, uint32_t vm, auto whole_step) {
+            constexpr bool FULL = decltype(whole_step)::value;
             // scores
-            float s[GS][NT][4];
+            float x[GS][NT][4];
 #pragma unroll
             for (int gi = 0; gi < GS; gi++) {
                 const uint8_t* gran = st + gi * L::GB;
@@ -339,98 +318,85 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
                         const uint32_t x0 = kw[0][gr][i], x1 = kw[1][gr][i], y0 = x0 >> 8, y1 = x1 >> 8;
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            const uint4 qb = *reinterpret_cast<const uint4*>(smem + L::Q +
-                                                                             ((nt * 8 + g) * D + gr * 64 + (2 * t + i) * 8) * 2);
+                            const uint4 qb = *reinterpret_cast<const uint4*>(q_lane + nt * 8 * D * 2 + (gr * 64 + i * 8) * 2);
                             mma16816(acc[gr][nt], x0 & 0x000f000fu, x1 & 0x000f000fu, y0 & 0x000f000fu, y1 & 0x000f000fu, qb.x, qb.y);
                             mma16816(acc[gr][nt], x0 & 0x00f000f0u, x1 & 0x00f000f0u, y0 & 0x00f000f0u, y1 & 0x00f000f0u, qb.z, qb.w);
                         }
                     }
                 }
+                float2 par[2][G];
+#pragma unroll
+                for (int rr = 0; rr < 2; rr++) load_params<G>(gran + kv4_kpar_off(D) + (tok0 + 8 * rr) * G * 4, par[rr]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) s[gi][nt][j] = 0.0f;
+                    for (int j = 0; j < 4; j++) {
+                        float v = par[j >> 1][0].y * qs[nt][j & 1][0];
+                        v = fmaf(par[j >> 1][0].x, acc[0][nt][j], v);
 #pragma unroll
-                for (int gr = 0; gr < G; gr++)
-#pragma unroll
-                    for (int rr = 0; rr < 2; rr++) {
-                        const __half2 par = *reinterpret_cast<const __half2*>(gran + kv4_kpar_off(D) + ((tok0 + 8 * rr) * G + gr) * 4);
-                        const float2 f = __half22float2(par);
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int j = 0; j < 2; j++)
-                                s[gi][nt][2 * rr + j] = fmaf(f.y, qs[nt][j][gr], fmaf(f.x, acc[gr][nt][2 * rr + j], s[gi][nt][2 * rr + j]));
-                    }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[gi][nt][j] *= chs[nt][j & 1];
-            }
-            if (!full) {
-#pragma unroll
-                for (int gi = 0; gi < GS; gi++)
-#pragma unroll
-                    for (int rr = 0; rr < 2; rr++) {
-                        const int key = p0 + gi * kKvGranule + tok0 + 8 * rr;
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int j = 0; j < 2; j++)
-                                if (!((vm >> gi) & 1u) || key >= r.hi || key > qpos[nt][j] ||
-                                    (a.window > 0 && key <= qpos[nt][j] - a.window))
-                                    s[gi][nt][2 * rr + j] = -CUDART_INF_F;
+                        for (int gr = 1; gr < G; gr++)
+                            v = fmaf(par[j >> 1][gr].x, acc[gr][nt][j], fmaf(par[j >> 1][gr].y, qs[nt][j & 1][gr], v));
+                        x[gi][nt][j] = v * chs[nt][j & 1];
                     }
             }
-
-            // the values' steps and minima of this lane's keys (0 for keys that no row sees)
-            float vs[GS][2][G], vmn[GS][2][G];
+            // the values' steps and minima of this lane's keys
+            float2 vpar[GS][2][G];
             float smax = 0.0f;
 #pragma unroll
             for (int gi = 0; gi < GS; gi++)
 #pragma unroll
                 for (int rr = 0; rr < 2; rr++) {
-                    const int key = p0 + gi * kKvGranule + tok0 + 8 * rr;
-                    const bool seen = full || (((vm >> gi) & 1u) && key < r.hi);
+                    load_params<G>(st + gi * L::GB + kv4_vpar_off(D) + (tok0 + 8 * rr) * G * 4, vpar[gi][rr]);
+                    if constexpr (!FULL) {
+                        // keys a column does not see score -inf; keys no row sees weigh 0 whatever they hold
+                        const int key = p0 + gi * kKvGranule + tok0 + 8 * rr;
+                        const bool here = ((vm >> gi) & 1u) && key < r.hi;
 #pragma unroll
-                    for (int gr = 0; gr < G; gr++) {
-                        const __half2 par =
-                            *reinterpret_cast<const __half2*>(st + gi * L::GB + kv4_vpar_off(D) + ((tok0 + 8 * rr) * G + gr) * 4);
-                        const float2 f = __half22float2(par);
-                        vs[gi][rr][gr] = seen ? f.x : 0.0f;
-                        vmn[gi][rr][gr] = seen ? f.y : 0.0f;
-                        smax = fmaxf(smax, vs[gi][rr][gr]);
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++)
+                                if (!here || key > qpos[nt][j] || (a.window > 0 && key <= qpos[nt][j] - a.window))
+                                    x[gi][nt][2 * rr + j] = -CUDART_INF_F;
+#pragma unroll
+                        for (int gr = 0; gr < G; gr++)
+                            if (!here) vpar[gi][rr][gr] = make_float2(0.0f, 0.0f);
                     }
+#pragma unroll
+                    for (int gr = 0; gr < G; gr++) smax = fmaxf(smax, vpar[gi][rr][gr].x);
                 }
-            float over = -CUDART_INF_F;
+            float best[NT][2];
+            bool move = smax > sthr;
 #pragma unroll
-            for (int gi = 0; gi < GS; gi++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int j = 0; j < 2; j++) {
+                    best[nt][j] = fmaxf(x[0][nt][j], x[0][nt][j + 2]);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) over = fmaxf(over, s[gi][nt][j] - mref[nt][j & 1]);
-            if (__any_sync(0xffffffffu, over > 15.0f - se || smax > sthr)) {
+                    for (int gi = 1; gi < GS; gi++) best[nt][j] = fmaxf(best[nt][j], fmaxf(x[gi][nt][j], x[gi][nt][j + 2]));
+                    move |= best[nt][j] > thr[nt][j];
+                }
+            if (__any_sync(0xffffffffu, move)) {
                 // move the references: each column's best score at 2^(11 - se)
 #pragma unroll
                 for (int m = 16; m > 0; m >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, m));
-                float se_new = se;
+                float grow = 0.0f;
                 if (smax > sthr) {
                     const int e = min(max((int)(__float_as_uint(smax) >> 23) - 126, -24), 17);
-                    se_new = (float)e;
+                    grow = lim - (15.0f - (float)e);
+                    lim = 15.0f - (float)e;
                     sthr = __uint_as_float((uint32_t)(e + 127) << 23);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        float best = -CUDART_INF_F;
+                        float top = best[nt][j];
 #pragma unroll
-                        for (int gi = 0; gi < GS; gi++) best = fmaxf(best, fmaxf(s[gi][nt][j], s[gi][nt][j + 2]));
-#pragma unroll
-                        for (int m = 4; m < 32; m <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, m));
-                        const float moved = fmaxf(mref[nt][j] + (se_new - se), best - (11.0f - se_new));
+                        for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+                        const float moved = fmaxf(mref[nt][j] + grow, top - (lim - 4.0f));
                         const float f = ex2(mref[nt][j] - moved);
                         mref[nt][j] = moved;
+                        thr[nt][j] = moved + lim;
                         l[nt][j] *= f;
 #pragma unroll
                         for (int gr = 0; gr < G; gr++) {
@@ -442,7 +408,6 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
                             }
                         }
                     }
-                se = se_new;
             }
 
             // probabilities and values
@@ -454,21 +419,22 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
                 for (int nt = 0; nt < NT; nt++) {
                     float p[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) p[j] = ex2(s[gi][nt][j] - mref[nt][j & 1]);
+                    for (int j = 0; j < 4; j++) p[j] = ex2(x[gi][nt][j] - mref[nt][j & 1]);
                     l[nt][0] += p[0] + p[2];
                     l[nt][1] += p[1] + p[3];
 #pragma unroll
                     for (int gr = 0; gr < G; gr++)
 #pragma unroll
                         for (int rr = 0; rr < 2; rr++) {
-                            float a0 = p[2 * rr] * vs[gi][rr][gr], a1 = p[2 * rr + 1] * vs[gi][rr][gr];
-                            float b0 = p[2 * rr] * vmn[gi][rr][gr], b1 = p[2 * rr + 1] * vmn[gi][rr][gr];
-                            if (!full) {  // a key one row sees and another does not may hold NaN
-                                if (p[2 * rr] == 0.0f) a0 = b0 = 0.0f;
-                                if (p[2 * rr + 1] == 0.0f) a1 = b1 = 0.0f;
+                            const float2 vp = vpar[gi][rr][gr];
+                            float a0 = p[2 * rr] * vp.x, a1 = p[2 * rr + 1] * vp.x;
+                            float b0 = p[2 * rr], b1 = p[2 * rr + 1], m0 = vp.y, m1 = vp.y;
+                            if constexpr (!FULL) {  // a key one row sees and another does not may hold NaN
+                                if (b0 == 0.0f) a0 = m0 = 0.0f;
+                                if (b1 == 0.0f) a1 = m1 = 0.0f;
                             }
-                            mn[gr][nt][0] += b0;
-                            mn[gr][nt][1] += b1;
+                            mn[gr][nt][0] = fmaf(b0, m0, mn[gr][nt][0]);
+                            mn[gr][nt][1] = fmaf(b1, m1, mn[gr][nt][1]);
                             const __half2 h2 = __floats2half2_rn(a0, a1);
                             pb[gr][nt][rr] = movmatrix(*reinterpret_cast<const uint32_t*>(&h2));
                         }
@@ -493,14 +459,21 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
                     const uint32_t w23[2] = {__byte_perm(vw[2][gr], vw[3][gr], 0x5410), __byte_perm(vw[2][gr], vw[3][gr], 0x7632)};
 #pragma unroll
                     for (int mt = 0; mt < 4; mt++) {
-                        const uint32_t x = w01[mt >> 1] >> (8 * (mt & 1)), y = w23[mt >> 1] >> (8 * (mt & 1));
+                        const uint32_t xx = w01[mt >> 1] >> (8 * (mt & 1)), yy = w23[mt >> 1] >> (8 * (mt & 1));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
-                            mma16816(o[gr][mt][nt], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u,
+                            mma16816(o[gr][mt][nt], xx & 0x000f000fu, xx & 0x00f000f0u, yy & 0x000f000fu, yy & 0x00f000f0u,
                                      pb[gr][nt][0], pb[gr][nt][1]);
                     }
                 }
             }
+        };
+        for (; mine < seg_end; mine += kStWarps) {
+            if (alive) alive = mbar_wait(&bar[stage], parity, DEV_TIMEOUT_FULL);
+            const int p0 = r.lo + (mine - cur.beg) * GS * kKvGranule;
+            const uint32_t vm = (valid >> (4 * stage)) & 15u;
+            if (p0 >= full_lo && p0 <= full_hi && vm == (1u << GS) - 1) step(ring + stage * L::STEP, p0, vm, std::true_type());
+            else step(ring + stage * L::STEP, p0, vm, std::false_type());
             __syncwarp();
             issue(stage);
             if (++stage == kStStages) stage = 0, parity ^= 1u;
@@ -523,8 +496,8 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
                 }
             }
         __syncthreads();
-        const bool whole = pos == cur.u0 && seg_end == cur.u0 + cur.n;
-        float* slot = a.part + (size_t)(2 * cta + (pos == start ? 0 : 1)) * (16 * (D + 2));
+        const bool whole = pos == cur.beg && seg_end == cur.beg + cur.n;
+        float* slot = a.part + (size_t)(2 * cta + (pos == 0 ? 0 : 1)) * (kStRows * (D + 2));
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -574,53 +547,13 @@ __global__ void __launch_bounds__(kStThreads, NT == 1 && D <= 128 ? 3 : 2) kv4_s
                     __stcg(dst, make_float4(v[0], v[1], v[2], v[3]));
                     __stcg(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
                     if (ch == 0) {
-                        __stcg(slot + 16 * D + 2 * c, top);
-                        __stcg(slot + 16 * D + 2 * c + 1, ls);
+                        __stcg(reinterpret_cast<float2*>(slot + kStRows * D + 2 * c), make_float2(top, ls));
                     }
                 }
             }
             __syncthreads();
         }
 
-        if (!whole) {
-            // CTAs first .. last share the unit; the first's counter counts them in
-            const int first = (int)(((cur.u0 + 1) * ctas - 1) / total);
-            const int last = (int)(((cur.u0 + cur.n) * ctas - 1) / total);
-            if (tid == 0) {
-                __threadfence();
-                arrived = atomicAdd(&a.count[first], 1);
-            }
-            __syncthreads();
-            if (arrived == last - first) {
-                __threadfence();
-                if (tid == 0) a.count[first] = 0;
-                const size_t stride = 16 * (D + 2);
-                auto slot_of = [&](int c) {
-                    return a.part + (size_t)(2 * c + (c == first && total * c / ctas != cur.u0 ? 1 : 0)) * stride;
-                };
-                for (int i = tid; i < ncols * (D / 4); i += kStThreads) {
-                    const int c = i / (D / 4), ch = (i % (D / 4)) * 4;
-                    float top = -1.0e30f;
-#pragma unroll 4
-                    for (int k = first; k <= last; k++) top = fmaxf(top, __ldcg(slot_of(k) + 16 * D + 2 * c));
-                    float ls = 0.0f;
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (int k = first; k <= last; k++) {
-                        const float* sl = slot_of(k);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(sl + 16 * D + 2 * c));
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(sl + c * D + ch));
-                        const float f = ex2(ml.x - top);
-                        ls += f * ml.y;
-                        v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
-                    }
-                    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-                    const size_t at = ((size_t)(r.q0 + c / a.group) * a.heads + cur.h * a.group + c % a.group) * D + ch;
-                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
-                        make_uint2(pack_act2(v.x * inv, v.y * inv, a.dt), pack_act2(v.z * inv, v.w * inv, a.dt));
-                }
-            }
-        }
         pos = seg_end;
     }
 }
@@ -629,8 +562,8 @@ namespace {
 
 template <int D, int NT>
 int stream_ctas() {
-    // CTAs an SM holds by shared memory (registers allow as many)
-    return std::min(4, (227 * 1024) / (StreamLayout<D, NT>::TOTAL + 1024)) * sm_count();
+    // CTAs an SM holds, by its shared memory and the kernel's launch bounds
+    return std::min(stream_resident<D, NT>(), (227 * 1024) / (StreamLayout<D, NT>::TOTAL + 1024)) * sm_count();
 }
 
 template <int D, int NT>
@@ -644,6 +577,13 @@ cudaError_t stream_launch(const Kv4AttnArgs& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int kv4_stream_grid(int D, int max_cols) {
+    const bool one = max_cols <= 8;
+    if (D == 64) return one ? stream_ctas<64, 1>() : stream_ctas<64, 2>();
+    if (D == 128) return one ? stream_ctas<128, 1>() : stream_ctas<128, 2>();
+    return one ? stream_ctas<256, 1>() : stream_ctas<256, 2>();
+}
 
 cudaError_t kv4_stream_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream) {
     const bool one = a.max_cols <= 8;

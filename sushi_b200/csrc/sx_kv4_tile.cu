@@ -14,8 +14,8 @@
 // products.  The reference moves only when a score passes it by 2^8 (P's best at 2^7, at most 2^15).
 //
 // Work: the units' tiles laid end to end and cut into equal runs, one a CTA (one CTA an SM), so
-// causal lengths balance and few long rows are split; a unit of several CTAs is joined by the last
-// to arrive, in CTA order.  Every wait is bounded (sx_common.cuh).
+// causal lengths balance and few long rows are split; a unit of several CTAs is joined by
+// sx_kv4_join.cu.  Every wait is bounded (sx_common.cuh).
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
@@ -29,8 +29,8 @@ constexpr int kTlDeqWarps = 4;
 template <int D>
 struct TileLayout {
     static constexpr int G = D / kKvGroup;
-    static constexpr int MT = D == 256 ? 1 : 2;
-    static constexpr int NK = D == 256 ? 64 : 128;
+    static constexpr int MT = kv4_tile_rows(D) / 128;
+    static constexpr int NK = kv4_tile_keys(D);
     static constexpr int KST = 2, VST = D == 256 ? 1 : 2;
     static constexpr int ROWS = 128 * MT;
     static constexpr int SM_WARPS = 4 * MT;
@@ -55,37 +55,12 @@ struct TileLayout {
     static_assert(ALLOC <= 227 * 1024, "fits a CTA");
 };
 
-// Block u of a request's (row, head) pairs: n tiles of keys from position lo.
-struct TileUnit {
-    int e0, rows;  // pairs [e0, e0 + rows)
-    int lo, n;
-};
-
-template <int D>
-__device__ __forceinline__ TileUnit tile_unit(const Kv4AttnArgs& a, const Kv4Request& r, int u) {
-    using L = TileLayout<D>;
-    TileUnit t;
-    t.e0 = u * L::ROWS;
-    t.rows = (int)min((long long)L::ROWS, r.qn * (long long)a.group - t.e0);
-    const int first = r.pos0 + t.e0 / a.group, last = r.pos0 + (t.e0 + t.rows - 1) / a.group;
-    const int hi = min(r.hi, last + 1);
-    t.lo = a.window > 0 ? max(0, min(first - a.window + 1, hi)) & ~(kKvGranule - 1) : 0;
-    t.n = hi > t.lo ? (hi - t.lo + L::NK - 1) / L::NK : 0;
-    return t;
-}
-
-// A request's blocks; 0 for the streaming kernel's requests.
-template <int D>
-__device__ __forceinline__ int tile_blocks(const Kv4AttnArgs& a, const Kv4Request& r) {
-    const long long pairs = r.qn * (long long)a.group;
-    return pairs <= a.max_cols ? 0 : (int)((pairs + TileLayout<D>::ROWS - 1) / TileLayout<D>::ROWS);
-}
-
+// A walk over the units' tiles: the unit's first tile is step `beg` of this CTA's run (negative where it
+// began in an earlier CTA's).
 struct TileCursor {
     Kv4Request r;
     TileUnit t;
-    int b, h, u, blocks;
-    long long u0;
+    int b, h, u, blocks, beg;
 };
 
 template <int D>
@@ -97,11 +72,11 @@ __device__ __forceinline__ void tile_load(const Kv4AttnArgs& a, TileCursor& c) {
     if (c.blocks) c.t = tile_unit<D>(a, c.r, 0);
 }
 
-// Moves the cursor forward to the unit that holds tile i of the list.
+// Moves the cursor forward to the unit that holds tile i of the run.
 template <int D>
-__device__ __forceinline__ void tile_seek(const Kv4AttnArgs& a, TileCursor& c, long long i) {
-    while (i >= c.u0 + c.t.n) {
-        c.u0 += c.t.n;
+__device__ __forceinline__ void tile_seek(const Kv4AttnArgs& a, TileCursor& c, int i) {
+    while (i >= c.beg + c.t.n) {
+        c.beg += c.t.n;
         if (++c.u >= c.blocks) {
             c.u = 0;
             if (++c.h >= a.kv_heads || c.blocks == 0) {
@@ -183,9 +158,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     constexpr int G = L::G, MT = L::MT, NK = L::NK;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_slot;
-    __shared__ long long red[L::THREADS / 32];
-    __shared__ int pick_b, arrived;
-    __shared__ long long pick_u0;
+    __shared__ int red[L::THREADS / 32], pick[2];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + L::BAR);  // [deq warps][RING]
@@ -208,14 +181,15 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
 
     // ---------------- the list's length; rows of blocks that see no key are zeroed here
     const size_t head_row = (size_t)a.heads * D;
-    auto request_tiles = [&](int b, bool zero) {
+    pdl_release();
+    auto steps = [&](int b) {
         const Kv4Request r = kv4_request(a, b);
         const int blocks = tile_blocks<D>(a, r);
-        long long n = 0;
+        int n = 0;
         for (int u = 0; u < blocks; u++) {
             const TileUnit t = tile_unit<D>(a, r, u);
             n += t.n;
-            if (zero && t.n == 0 && (b + u) % (int)gridDim.x == (int)blockIdx.x)
+            if (t.n == 0 && (b + u) % (int)gridDim.x == (int)blockIdx.x)
                 for (int h = 0; h < a.kv_heads; h++)
                     for (int e = t.e0; e < t.e0 + t.rows; e++) {
                         uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + e / a.group) * head_row +
@@ -225,41 +199,18 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
         }
         return n * a.kv_heads;
     };
-    long long total = 0;
-    for (int b = tid; b < a.requests; b += L::THREADS) total += request_tiles(b, true);
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
-    if (lane == 0) red[warp] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < L::THREADS / 32; w++) total += red[w];
-    const long long ctas = min((long long)gridDim.x, total);
+    constexpr int W = L::THREADS / 32;
+    int n0;
+    const int total = list_total<W>(a.requests, red, n0, steps);
+    const RunCut run(total, gridDim.x);
     const int cta = blockIdx.x;
-    if (cta >= ctas) return;
-    const long long start = total * cta / ctas, end = total * (cta + 1) / ctas;
-    long long base = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += L::THREADS) {
-        const int b = b0 + tid;
-        const long long n = b < a.requests ? request_tiles(b, false) : 0;
-        long long s = n;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, s, m);
-            if (lane >= m) s += x;
-        }
-        __syncthreads();
-        if (lane == 31) red[warp] = s;
-        __syncthreads();
-        long long all = 0;
-        for (int w = 0; w < L::THREADS / 32; w++) {
-            if (w < warp) s += red[w];
-            all += red[w];
-        }
-        if (n > 0 && start >= base + s - n && start < base + s) pick_b = b, pick_u0 = base + s - n;
-        base += all;
-        if (start < base) break;
+    if (total == 0 || cta >= run.ctas) {
+        pdl_wait();  // the join that follows waits for this grid: the streaming kernel's end is part of it
+        return;
     }
+    const int start = run.start(cta);
+    const int len = run.start(cta + 1) - start;  // this CTA's run
+    list_find<W>(a.requests, red, pick, n0, start, steps);
     if (warp == L::SM_WARPS + kTlDeqWarps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512)
                      : "memory");
@@ -270,8 +221,8 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     TileCursor cur;
-    cur.b = pick_b;
-    cur.u0 = pick_u0;
+    cur.b = pick[0];
+    cur.beg = pick[1] - start;
     tile_load<D>(a, cur);
 
     if (warp < L::SM_WARPS) {
@@ -282,14 +233,14 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
         uint32_t turns = 0;   // tiles this row tile has taken
         uint32_t tiles = 0;   // tiles the CTA has taken (the value ring's turn)
         bool ok = true;
-        for (long long pos = start; pos < end;) {
+        for (int pos = 0; pos < len;) {
             // both row tiles start a unit together: one that sits a unit out must not count for the next
             asm volatile("bar.sync 2, %0;" ::"n"(L::SM_WARPS * 32) : "memory");
             tile_seek<D>(a, cur, pos);
             const Kv4Request r = cur.r;
             const TileUnit un = cur.t;
-            const long long seg_end = min(end, cur.u0 + un.n);
-            const int j0 = (int)(pos - cur.u0), n = (int)(seg_end - pos);
+            const int seg_end = min(len, cur.beg + un.n);
+            const int j0 = pos - cur.beg, n = seg_end - pos;
             const int e = mt * 128 + row;
             const bool live = e < un.rows;                    // this thread has a pair
             const bool tile_live = mt * 128 < un.rows;        // the row tile takes part
@@ -455,7 +406,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
 
             // ---------------- the rows out, or this CTA's share of them into its slot
             const bool whole = j0 == 0 && n == un.n;
-            float* slot = a.part + (size_t)(2 * cta + (pos == start ? 0 : 1)) * (L::ROWS * (D + 2));
+            float* slot = a.part + (size_t)(2 * cta + (pos == 0 ? 0 : 1)) * (L::ROWS * (D + 2));
             if (tile_live) {
                 if (ok) ok = mbar_wait(&odone[MT == 2 ? mt : 0], (turns - 1) & 1, DEV_TIMEOUT_FULL);
                 tc_fence_after();
@@ -491,44 +442,6 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                 if (!whole && live)
                     __stcg(reinterpret_cast<float2*>(slot + L::ROWS * D + 2 * e), make_float2(mref, l));
             }
-            if (!whole) {
-                constexpr int NT = L::SM_WARPS * 32;
-                const int firstc = (int)(((cur.u0 + 1) * ctas - 1) / total);
-                const int lastc = (int)(((cur.u0 + un.n) * ctas - 1) / total);
-                __threadfence();
-                asm volatile("bar.sync 2, %0;" ::"n"(NT) : "memory");
-                if (tid == 0) arrived = atomicAdd(&a.count[firstc], 1);
-                asm volatile("bar.sync 2, %0;" ::"n"(NT) : "memory");
-                if (arrived == lastc - firstc) {
-                    __threadfence();
-                    if (tid == 0) a.count[firstc] = 0;
-                    auto slot_of = [&](int k) {
-                        return a.part + (size_t)(2 * k + (k == firstc && total * k / ctas != cur.u0 ? 1 : 0)) * (L::ROWS * (D + 2));
-                    };
-                    for (int i = tid; i < un.rows * (D / 4); i += NT) {
-                        const int ee = i / (D / 4), ch = (i % (D / 4)) * 4;
-                        float best = -1.0e30f;
-#pragma unroll 4
-                        for (int k = firstc; k <= lastc; k++) best = fmaxf(best, __ldcg(slot_of(k) + L::ROWS * D + 2 * ee));
-                        float ls = 0.0f;
-                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                        for (int k = firstc; k <= lastc; k++) {
-                            const float* sl = slot_of(k);
-                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(sl + L::ROWS * D + 2 * ee));
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(sl + ee * D + ch));
-                            const float f = ex2(ml.x - best);
-                            ls += f * ml.y;
-                            v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
-                        }
-                        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-                        const int p = un.e0 + ee;
-                        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (r.q0 + p / a.group) * head_row +
-                                                  (size_t)(cur.h * a.group + p % a.group) * D + ch) =
-                            make_uint2(pack_act2(v.x * inv, v.y * inv, a.dt), pack_act2(v.z * inv, v.w * inv, a.dt));
-                    }
-                }
-            }
             pos = seg_end;
         }
     } else if (warp < L::SM_WARPS + kTlDeqWarps) {
@@ -539,12 +452,12 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
         uint32_t tiles = 0, taken = 0;  // tiles widened, granules consumed
         uint32_t there = 0;             // a bit a ring place: the granule was copied
         bool ok = true;
-        for (long long pos = start; pos < end;) {
+        for (int pos = 0; pos < len;) {
             tile_seek<D>(a, cur, pos);
             const Kv4Request r = cur.r;
-            const long long seg_end = min(end, cur.u0 + cur.t.n);
-            const int n = (int)(seg_end - pos);
-            const int lo = cur.t.lo + (int)(pos - cur.u0) * NK;
+            const int seg_end = min(len, cur.beg + cur.t.n);
+            const int n = seg_end - pos;
+            const int lo = cur.t.lo + (pos - cur.beg) * NK;
             auto issue = [&](int q) {  // granule q of the warp's share of the segment, into place (taken + q) % RING
                 const int key = lo + (q / L::GPW) * NK + (w * L::GPW + q % L::GPW) * kKvGranule;
                 const int place = (int)((taken + q) % L::RING);
@@ -686,10 +599,10 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             }
             tc_commit(&odone[MT == 2 ? mt : 0]);
         };
-        for (long long pos = start; pos < end;) {
+        for (int pos = 0; pos < len;) {
             tile_seek<D>(a, cur, pos);
-            const long long seg_end = min(end, cur.u0 + cur.t.n);
-            const int n = (int)(seg_end - pos);
+            const int seg_end = min(len, cur.beg + cur.t.n);
+            const int n = seg_end - pos;
             const int live = MT == 2 && cur.t.rows > 128 ? 2 : 1;
             if (ok) ok = mbar_wait(qfull, segs & 1, DEV_TIMEOUT_FULL);
             if (ok) ok = mbar_wait(&kfull[tiles % L::KST], (tiles / L::KST) & 1, DEV_TIMEOUT_FULL);
@@ -728,6 +641,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
         // the last commit of all: nothing of this CTA's is in flight when it frees its tensor memory
         if (ok) mbar_wait(&vempty[(tiles - 1) % L::VST], ((tiles - 1) / L::VST) & 1, DEV_TIMEOUT_EMPTY);
     }
+    pdl_wait();  // the join that follows waits for this grid: the streaming kernel's end is part of it
     tc_fence_before();
     __syncthreads();
     if (warp == L::SM_WARPS + kTlDeqWarps) {
@@ -744,13 +658,21 @@ cudaError_t tile_launch(const Kv4AttnArgs& a, cudaStream_t stream) {
     auto kern = kv4_tile_kernel<D>;
     cudaError_t e = func_attrs(reinterpret_cast<const void*>(kern), L::ALLOC, false);
     if (e != cudaSuccess) return e;
-    kern<<<sm_count(), L::THREADS, L::ALLOC, stream>>>(a);
-    return cudaGetLastError();
+    // starts as the streaming kernel drains: neither reads what the other writes
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sm_count(), 1, 1);
+    cfg.blockDim = dim3(L::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = L::ALLOC;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 }  // namespace
-
-size_t kv4_tile_part_floats(int D) { return (size_t)(D == 256 ? 128 : 256) * (D + 2); }
 
 cudaError_t kv4_tile_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream) {
     if (D == 64) return tile_launch<64>(a, stream);

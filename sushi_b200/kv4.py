@@ -16,7 +16,14 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .exl3 import _DT, Exl3Error, _check, _stream, lib
+from .exl3 import _DT, Exl3Error, _check, lib
+
+_I32, _I64, _U8 = torch.int32, torch.int64, torch.uint8
+
+
+def _stream(device):
+    """The current stream's handle on `device` (as an int: no Stream object a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class Kv4Cache:
@@ -36,9 +43,11 @@ class Kv4Cache:
         elif pool.numel() != self.pages * self.kv_heads * block or not pool.is_contiguous() or not pool.is_cuda:
             raise Exl3Error(1)
         self.pool = pool
+        self._c = _lib.SxKv4(pool.data_ptr(), self.pages, self.kv_heads, self.head_dim, self.page_size)
+        self._ref = ctypes.byref(self._c)
 
     def c(self):
-        return _lib.SxKv4(self.pool.data_ptr(), self.pages, self.kv_heads, self.head_dim, self.page_size)
+        return self._c
 
 
 class BlockTables(NamedTuple):
@@ -51,8 +60,8 @@ class BlockTables(NamedTuple):
     free_left: torch.Tensor  # [1] int32
 
 
-def _ints(t, n=None, dtype=torch.int32):
-    if t.dtype != dtype:
+def _ints(t, n=None, dtype=_I32):
+    if t.dtype is not dtype:
         raise Exl3Error(2)
     if not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise Exl3Error(1)
@@ -60,11 +69,14 @@ def _ints(t, n=None, dtype=torch.int32):
 
 
 def _table(table, requests):
-    if table.dtype != torch.int32:
+    if table.dtype is not _I32:
         raise Exl3Error(2)
-    if not table.is_cuda or table.dim() != 2 or table.shape[0] != requests or table.shape[1] < 1 or table.stride(1) != 1:
+    if not table.is_cuda or table.dim() != 2:
         raise Exl3Error(1)
-    return table.data_ptr(), table.shape[1], max(table.stride(0), table.shape[1]) if requests == 1 else table.stride(0)
+    (rows, width), (stride, inner) = table.shape, table.stride()
+    if rows != requests or width < 1 or (inner != 1 and width > 1):
+        raise Exl3Error(1)
+    return table.data_ptr(), width, max(stride, width) if rows == 1 else stride
 
 
 def block_tables(ctx_lens, new_lens, table, free_pages, free_count, page_size: int, tokens: int) -> BlockTables:
@@ -76,24 +88,28 @@ def block_tables(ctx_lens, new_lens, table, free_pages, free_count, page_size: i
     c, n = _ints(ctx_lens), _ints(new_lens, requests)
     t, width, stride = _table(table, requests)
     f, fc = _ints(free_pages), _ints(free_count, 1)
-    i32 = dict(dtype=torch.int32, device=ctx_lens.device)
     tokens = int(tokens)
     if tokens < 0:
         raise Exl3Error(1)
-    out = BlockTables(torch.empty(requests, **i32), torch.empty(requests + 1, **i32),
-                      torch.empty(tokens, dtype=torch.int64, device=ctx_lens.device), torch.empty(tokens, **i32),
-                      torch.empty(1, **i32))
-    _check(lib().sx_block_tables(_stream(), c, n, requests, int(page_size), t, width, stride, f, fc, tokens,
-                                 *(x.data_ptr() for x in out)))
-    return out
+    # one buffer for the five outputs: slots (64-bit) first
+    buf = ctx_lens.new_empty(3 * tokens + 2 * requests + 2)
+    slots, positions, kv_lens, cu_q, left = buf.split_with_sizes([2 * tokens, tokens, requests, requests + 1, 1])
+    p = buf.data_ptr()
+    _check(lib().sx_block_tables(_stream(buf.device), c, n, requests, page_size, t, width, stride, f, fc, tokens,
+                                 p + 12 * tokens, p + 12 * tokens + 4 * requests, p, p + 8 * tokens,
+                                 p + 12 * tokens + 8 * requests + 4))
+    return BlockTables(kv_lens, cu_q, slots.view(_I64), positions, left)
 
 
 def _rows(x, heads, head_dim):
     if x.dtype not in _DT:
         raise Exl3Error(2)
-    if not x.is_cuda or x.dim() != 3 or x.shape[1] != heads or x.shape[2] != head_dim or x.stride(2) != 1:
+    if not x.is_cuda or x.dim() != 3:
         raise Exl3Error(1)
-    return x.data_ptr(), x.stride(0), x.stride(1)
+    (_, h, d), (ts, hs, inner) = x.shape, x.stride()
+    if h != heads or d != head_dim or inner != 1:
+        raise Exl3Error(1)
+    return x.data_ptr(), ts, hs
 
 
 def kv4_write(cache: Kv4Cache, k, v, slots):
@@ -104,9 +120,9 @@ def kv4_write(cache: Kv4Cache, k, v, slots):
         raise Exl3Error(2)
     if v.shape[0] != k.shape[0]:
         raise Exl3Error(1)
-    s = _ints(slots, k.shape[0], torch.int64)
-    c = cache.c()
-    _check(lib().sx_kv4_write(_stream(), ctypes.byref(c), *kp, *vp, _DT[k.dtype], k.shape[0], s))
+    tokens = k.shape[0]
+    s = _ints(slots, tokens, _I64)
+    _check(lib().sx_kv4_write(_stream(k.device), cache._ref, *kp, *vp, _DT[k.dtype], tokens, s))
 
 
 def kv4_read(cache: Kv4Cache, slots, dtype=torch.bfloat16):
@@ -114,33 +130,29 @@ def kv4_read(cache: Kv4Cache, slots, dtype=torch.bfloat16):
     two [tokens, kv_heads, head_dim] tensors (zeros where a slot is -1)."""
     if dtype not in _DT:
         raise Exl3Error(2)
-    s = _ints(slots, dtype=torch.int64)
+    s = _ints(slots, dtype=_I64)
     n = slots.numel()
-    k = torch.empty((n, cache.kv_heads, cache.head_dim), dtype=dtype, device=slots.device)
-    v = torch.empty_like(k)
-    c = cache.c()
-    _check(lib().sx_kv4_read(_stream(), ctypes.byref(c), s, n, _DT[dtype], k.data_ptr(), v.data_ptr()))
+    kv = slots.new_empty((2, n, cache.kv_heads, cache.head_dim), dtype=dtype)
+    k, v = kv.unbind()
+    _check(lib().sx_kv4_read(_stream(kv.device), cache._ref, s, n, _DT[dtype], k.data_ptr(), v.data_ptr()))
     return k, v
 
 
 def kv4_attention_workspace_bytes(cache: Kv4Cache, requests: int, tokens: int, heads: int, max_q: int) -> int:
-    c = cache.c()
-    return lib().sx_kv4_attention_workspace_bytes(ctypes.byref(c), int(requests), int(tokens), int(heads), int(max_q))
+    return lib().sx_kv4_attention_workspace_bytes(cache._ref, int(requests), int(tokens), int(heads), int(max_q))
 
 
 _WS = {}
 
 
-def _workspace(nbytes, device):
-    """The zeroed workspace of the current stream (every call leaves it zeroed, so it is kept).  While
-    a graph is being recorded a fresh one is made inside it: memory the recording only plans to zero
-    must not serve calls outside."""
+def _workspace(nbytes, device, stream):
+    """The workspace of a stream, kept for its next calls; inside a graph recording one of the graph's own."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+        return torch.empty(nbytes, dtype=_U8, device=device)
+    key = (device.index, stream)
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _WS[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        ws = _WS[key] = torch.empty(nbytes, dtype=_U8, device=device)
     return ws
 
 
@@ -150,22 +162,24 @@ def kv4_attention(q, cache: Kv4Cache, table, kv_lens, cu_q, max_q: int, scale=No
     Request b's rows are cu_q[b]..cu_q[b+1] (at most max_q), its keys the kv_lens[b] tokens its row
     of `table` [requests, width] names, the step's own last; causal, with a sliding window of
     `window` positions when it is positive.  scale: head_dim**-0.5 when None.  out: an optional
-    contiguous tensor of q's shape and dtype.  workspace: an optional zeroed uint8 tensor of
-    kv4_attention_workspace_bytes(...) bytes, reused across calls on one stream."""
+    contiguous tensor of q's shape and dtype.  workspace: an optional uint8 tensor of
+    kv4_attention_workspace_bytes(...) bytes, for the calls of one stream."""
     if q.dim() != 3:
         raise Exl3Error(1)
-    qp, ts, hs = _rows(q, q.shape[1], cache.head_dim)
+    tokens, heads, _ = q.shape
+    qp, ts, hs = _rows(q, heads, cache.head_dim)
     requests = kv_lens.numel()
     kl, cu = _ints(kv_lens), _ints(cu_q, requests + 1)
     t, width, stride = _table(table, requests)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise Exl3Error(1)
-    c = cache.c()
-    need = lib().sx_kv4_attention_workspace_bytes(ctypes.byref(c), requests, q.shape[0], q.shape[1], int(max_q))
-    ws = workspace if workspace is not None else _workspace(max(need, 16), q.device)
-    _check(lib().sx_kv4_attention(_stream(), ctypes.byref(c), qp, ts, hs, _DT[q.dtype], q.shape[0], q.shape[1], cu, kl, t,
-                                  requests, width, stride, int(max_q), cache.head_dim ** -0.5 if scale is None else float(scale),
-                                  int(window), out.data_ptr(), ws.data_ptr(), ws.numel()))
+    L, st = lib(), _stream(q.device)
+    if workspace is None:
+        need = L.sx_kv4_attention_workspace_bytes(cache._ref, requests, tokens, heads, max_q)
+        workspace = _workspace(max(need, 16), q.device, st)
+    _check(L.sx_kv4_attention(st, cache._ref, qp, ts, hs, _DT[q.dtype], tokens, heads, cu, kl, t, requests, width, stride,
+                              max_q, cache.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
+                              workspace.data_ptr(), workspace.numel()))
     return out

@@ -69,6 +69,7 @@ def test_cache_refusals(L, kw, want):
         (dict(requests=0), "SX_ERR_BAD_SHAPE"),
         (dict(width=0), "SX_ERR_BAD_SHAPE"),
         (dict(stride=3), "SX_ERR_BAD_SHAPE"),
+        (dict(requests=1 << 20, width=1 << 10, stride=1 << 10), "SX_ERR_BAD_SHAPE"),
         (dict(max_q=0), "SX_ERR_BAD_SHAPE"),
         (dict(window=-1), "SX_ERR_BAD_SHAPE"),
         (dict(scale=float("nan")), "SX_ERR_BAD_SHAPE"),
