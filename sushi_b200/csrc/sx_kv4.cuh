@@ -1,9 +1,10 @@
 // The 4-bit key/value cache: where a block keeps each code and parameter.
 //
 // A block (one page of one head) is page_size/16 granules of 16 tokens, each contiguous:
-//   [16 x D/2 key codes][16 x D/2 value codes][16 x G key parameters][16 x G value parameters]
+//   [16 x D/2 key codes][16 x G key parameters][16 x D/2 value codes][16 x G value parameters]
 // (G = D/64 groups; a parameter is the F16 step in the low half and the F16 minimum in the high
-// half of a 32-bit word), so one bulk copy brings a granule, keys and values, into shared memory.
+// half of a 32-bit word), so one bulk copy brings a granule, or its keys or values alone, into shared
+// memory.
 // A code row is D/8 words of eight consecutive channels, channel c in nibble c % 8 of its word.
 // The words of a row are ordered for the attention kernel's shared-memory reads:
 //   keys:   a lane (token row g, t = 0..3) of an m16n8k16 A fragment takes words 2t and 2t+1 of every
@@ -28,9 +29,9 @@ constexpr float kKvLargest = 57344.0f;
 constexpr int kKvGranule = 16;  // tokens of one contiguous piece of a block
 
 __host__ __device__ constexpr int kv4_granule_bytes(int D) { return kKvGranule * (D + 8 * (D / kKvGroup)); }
-__host__ __device__ constexpr int kv4_value_off(int D) { return kKvGranule * D / 2; }
-__host__ __device__ constexpr int kv4_kpar_off(int D) { return kKvGranule * D; }
-__host__ __device__ constexpr int kv4_vpar_off(int D) { return kKvGranule * (D + 4 * (D / kKvGroup)); }
+__host__ __device__ constexpr int kv4_kpar_off(int D) { return kKvGranule * D / 2; }
+__host__ __device__ constexpr int kv4_value_off(int D) { return kv4_granule_bytes(D) / 2; }
+__host__ __device__ constexpr int kv4_vpar_off(int D) { return kv4_value_off(D) + kKvGranule * D / 2; }
 
 // Byte offset in a granule of the key word (group gr, word w of 8) of token tok (0..15).
 template <int D>

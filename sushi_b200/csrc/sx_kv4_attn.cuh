@@ -172,6 +172,62 @@ __device__ __forceinline__ void list_find(int requests, int* red, int* pick, int
     __syncthreads();
 }
 
+// The tile kernel's list, W warps together: every request's tiles (over one key head), by a warp a request
+// where requests are few (their blocks are many then), else by a thread; `each` sees every unit once.
+constexpr int kTlFew = 64;
+template <int D, int W, typename F>
+__device__ __forceinline__ int tile_list_total(const Kv4AttnArgs& a, int* red, int* few, int& n0, F each) {
+    auto request = [&](int b, int u0, int du) {
+        const Kv4Request r = kv4_request(a, b);
+        const int blocks = tile_blocks<D>(a, r);
+        int n = 0;
+        for (int u = u0; u < blocks; u += du) {
+            const TileUnit t = tile_unit<D>(a, r, u);
+            each(b, r, t, u);
+            n += t.n;
+        }
+        return n;
+    };
+    if (a.requests <= kTlFew) {
+        for (int b = threadIdx.x >> 5; b < a.requests; b += W) {
+            const int n = __reduce_add_sync(0xffffffffu, request(b, threadIdx.x & 31, 32));
+            if ((threadIdx.x & 31) == 0) few[b] = n * a.kv_heads;
+        }
+        __syncthreads();
+        return list_total<W>(a.requests, red, n0, [&](int b) { return few[b]; });
+    }
+    return list_total<W>(a.requests, red, n0, [&](int b) { return request(b, 0, 1) * a.kv_heads; });
+}
+
+// The unit that holds step `at` of the list: request pick[0], block pick[2], key head pick[4]; its first
+// step is list position pick[3] (pick[1]: the request's).
+template <int D, int W>
+__device__ __forceinline__ void tile_list_find(const Kv4AttnArgs& a, int* red, int* pick, int n0, int at) {
+    list_find<W>(a.requests, red, pick, n0, at, [&](int b) {
+        const Kv4Request r = kv4_request(a, b);
+        const int blocks = tile_blocks<D>(a, r);
+        int n = 0;
+        for (int u = 0; u < blocks; u++) n += tile_unit<D>(a, r, u).n;
+        return n * a.kv_heads;
+    });
+    const Kv4Request r = kv4_request(a, pick[0]);
+    const int blocks = tile_blocks<D>(a, r);
+    auto unit = [&](int u) { return u < blocks ? tile_unit<D>(a, r, u).n : 0; };
+    int head = 0, before;
+    for (int u0 = 0; u0 < blocks; u0 += W * 32) head += block_scan<W>(unit(u0 + threadIdx.x), red, before);
+    const int h = (at - pick[1]) / head, first = pick[1] + h * head;
+    int base = first;
+    for (int u0 = 0; u0 < blocks; u0 += W * 32) {
+        const int n = unit(u0 + threadIdx.x);
+        const int all = block_scan<W>(n, red, before);
+        before += base;
+        if (n > 0 && at >= before && at < before + n) pick[2] = u0 + threadIdx.x, pick[3] = before, pick[4] = h;
+        base += all;
+        if (at < base) break;
+    }
+    __syncthreads();
+}
+
 // Programmatic dependent launch: the next kernel of the call may start; this one's predecessors done.
 __device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -20,7 +20,7 @@ constexpr int kJoinShares = 64;  // shares whose weights are held at a time
 
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, Kv4AttnArgs ta, int stream_grid, int tile_grid) {
-    __shared__ int red[kJoinWarps], pick[2];
+    __shared__ int red[kJoinWarps], pick[5], few[kTlFew];
     __shared__ float top_sm[kJoinRows], inv_sm[kJoinRows];
     __shared__ float wt[kJoinRows * kJoinShares];
     __shared__ float4 part_sm[kJoinThreads];
@@ -31,16 +31,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
     const int row0 = tile ? ((int)blockIdx.x - (stream_grid - 1)) % TG * kJoinRows : 0;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-    auto steps = [&](int b) {
-        const Kv4Request r = kv4_request(a, b);
-        if (!tile) return stream_steps<D>(a, r) * a.kv_heads;
-        int n = 0;
-        const int blocks = tile_blocks<D>(a, r);
-        for (int u = 0; u < blocks; u++) n += tile_unit<D>(a, r, u).n;
-        return n * a.kv_heads;
-    };
+    auto steps = [&](int b) { return stream_steps<D>(a, kv4_request(a, b)) * a.kv_heads; };
     int n0;
-    const int total = list_total<kJoinWarps>(a.requests, red, n0, steps);
+    const int total = tile ? tile_list_total<D, kJoinWarps>(a, red, few, n0, [](int, const Kv4Request&, const TileUnit&, int) {})
+                           : list_total<kJoinWarps>(a.requests, red, n0, steps);
     const RunCut run(total, tile ? tile_grid : stream_most(total, stream_grid));
     // A CTA with nothing to join waits too: this grid's end stands for the whole call's.
     if (total == 0 || cut >= run.ctas) {
@@ -48,9 +42,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
         return;
     }
     const int at = run.start(cut);
-    list_find<kJoinWarps>(a.requests, red, pick, n0, at, steps);
-    const int b = pick[0];
-    const Kv4Request r = kv4_request(a, b);
+    if (tile) tile_list_find<D, kJoinWarps>(a, red, pick, n0, at);
+    else list_find<kJoinWarps>(a.requests, red, pick, n0, at, steps);
+    const Kv4Request r = kv4_request(a, pick[0]);
     int h, u0, n, e0 = 0, rows;
     if (!tile) {
         n = stream_steps<D>(a, r);
@@ -58,14 +52,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
         u0 = pick[1] + h * n;
         rows = r.qn * a.group;
     } else {
-        const int head = steps(b) / a.kv_heads;  // tiles a key head
-        h = (at - pick[1]) / head;
-        u0 = pick[1] + h * head;
-        TileUnit t = tile_unit<D>(a, r, 0);
-        for (int u = 0; at >= u0 + t.n;) {
-            u0 += t.n;
-            t = tile_unit<D>(a, r, ++u);
-        }
+        const TileUnit t = tile_unit<D>(a, r, pick[2]);
+        u0 = pick[3], h = pick[4];
         n = t.n, e0 = t.e0, rows = t.rows;
     }
     const int first = run.owner(u0);

@@ -6,12 +6,13 @@
 //   S = Q K^T  (tcgen05, M = 128, N = NK, both from shared memory, f32 in tensor memory)
 //   P = exp2(c S - ref) by one thread a row, F16, over S's columns in tensor memory
 //   O += P V   (tcgen05, A = P from tensor memory, B = V from shared memory)
-// Four warps widen the codes to F16 tiles, key and value alike (code * s + m, rounded once: one word
-// of eight codes is one 16-byte chunk), from granules that bulk copies bring.  Eight consecutive
-// channels lie in the order of a word's nibble pairs (0 4 1 5 2 6 3 7), in Q and K alike, and in O's
-// columns.  Keys are K-major (rows of 64 channels, 128-byte swizzle); values have the same image,
-// read as the N-major operand.  The two row tiles take turns: one's softmax runs under the other's
-// products.  The reference moves only when a score passes it by 2^8 (P's best at 2^7, at most 2^15).
+// Other warps widen the codes to F16 tiles (code * s + m, rounded once: one word of eight codes is one
+// 16-byte chunk): a task is the keys or the values of one granule; the warps take them in turn, each from
+// its own ring of bulk copies.  Eight consecutive channels lie in the order of a word's nibble pairs
+// (0 4 1 5 2 6 3 7), in Q and K alike, and in O's columns.  Keys are K-major (rows of 64 channels,
+// 128-byte swizzle); values have the same image, read as the N-major operand.  The two row tiles take
+// turns: one's softmax runs under the other's products.  The reference moves only when a score passes
+// it by 2^8 (P's best at 2^7, at most 2^15).
 //
 // Work: the units' tiles laid end to end and cut into equal runs, one a CTA (one CTA an SM), so
 // causal lengths balance and few long rows are split; a unit of several CTAs is joined by
@@ -24,20 +25,23 @@
 
 namespace sx {
 
-constexpr int kTlDeqWarps = 4;
-
 template <int D>
 struct TileLayout {
     static constexpr int G = D / kKvGroup;
     static constexpr int MT = kv4_tile_rows(D) / 128;
     static constexpr int NK = kv4_tile_keys(D);
+    static constexpr int NG = NK / kKvGranule;  // granules a tile
     static constexpr int KST = 2, VST = D == 256 ? 1 : 2;
-    static constexpr int ROWS = 128 * MT;
+    // Widening warps.  7 beside 8 softmax warps and the MMA warp: 16, so 128 registers a thread.  Every
+    // warp must have a task among a tile's keys (and among its values) in every tile or in none: a wait by
+    // parity tells only neighbouring phases of a stage apart.
+    static constexpr int WIDEN = D == 256 ? 8 : 7;
+    static_assert(WIDEN <= NG || WIDEN == 2 * NG, "no warp passes over a tile's stage");
     static constexpr int SM_WARPS = 4 * MT;
-    static constexpr int THREADS = (SM_WARPS + kTlDeqWarps + 1) * 32;
-    static constexpr int GB = kv4_granule_bytes(D);
-    static constexpr int GPW = NK / kKvGranule / kTlDeqWarps;  // granules a warp a tile
-    static constexpr int RING = D == 128 ? 3 : (D == 64 ? 4 : 2);
+    static constexpr int MMA_WARP = SM_WARPS + WIDEN;
+    static constexpr int THREADS = (MMA_WARP + 1) * 32;
+    static constexpr int HB = kv4_granule_bytes(D) / 2;  // a granule's keys, or its values
+    static constexpr int RING = D == 128 ? 3 : (D == 64 ? 6 : 2);
     static constexpr int Q_TILE = 128 * D * 2;
     static constexpr int KV_TILE = NK * D * 2;
     static constexpr int SUB = NK * 128;  // bytes of 64 channels of a key tile
@@ -45,9 +49,10 @@ struct TileLayout {
     static constexpr int K = Q + MT * Q_TILE;
     static constexpr int V = K + KST * KV_TILE;
     static constexpr int RAW = V + VST * KV_TILE;
-    static constexpr int BAD = RAW + kTlDeqWarps * RING * GB;  // [VST][G][NK / 16] u16
-    static constexpr int BAR = (BAD + VST * G * (NK / 16) * 2 + 15) / 16 * 16;
-    static constexpr int NBAR = kTlDeqWarps * RING + 2 * KST + 2 * VST + 2 + 2 + 2 + 1;
+    static constexpr int BAD = RAW + WIDEN * RING * HB;  // [VST][G][NG] u16: keys whose value group holds NaN
+    static constexpr int GONE = BAD + VST * G * NG * 2;     // [4][NG] u8: granules without a page
+    static constexpr int BAR = (GONE + 4 * NG + 15) / 16 * 16;
+    static constexpr int NBAR = WIDEN * RING + 2 * KST + 2 * VST + 2 + 2 + 2 + 1;
     static constexpr int TOTAL = BAR + NBAR * 8;
     static constexpr int ALLOC = TOTAL + 1024;
     static constexpr int S_COL = 0;  // two S tiles of NK columns
@@ -105,22 +110,46 @@ __device__ __forceinline__ uint64_t smem_desc_sw128_n(uint32_t saddr, uint32_t l
            (uint64_t)1u << 46 | (uint64_t)2u << 61;
 }
 
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+// 32 columns of this warp's 32 lanes, in two parts: a load is in flight while the one before is worked on.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+        "%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t (&r)[32]) {  // names the registers: nothing reads them earlier
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+        "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+        "%28,%29,%30,%31,%32};" ::"r"(taddr),
+          "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+          "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
 
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-    uint32_t r[16];
+    uint32_t r[32];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) r[i] = __float_as_uint(v[h * 16 + i]);
-        tmem_st16(taddr + h * 16, r);
-    }
+    for (int i = 0; i < 32; i++) r[i] = __float_as_uint(v[i]);
+    tmem_st32u(taddr, r);
 }
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -152,17 +181,110 @@ __device__ __forceinline__ __half2 as_half2(uint32_t p) { return *reinterpret_ca
 // The channel of eight that sits at place p of a chunk.
 __host__ __device__ constexpr int chunk_channel(int p) { return (p >> 1) + 4 * (p & 1); }
 
+// The keys of a granule as rows row0 .. row0 + 15 of a tile; tokens from `live` on become 0.  Lanes: words
+// 2t and 2t + 1 of every group of one token, eight tokens at a time.
+template <int D>
+__device__ __forceinline__ void widen_keys(const uint8_t* gran, int live, int row0, uint8_t* out) {
+    using L = TileLayout<D>;
+    constexpr int G = L::G;
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    uint32_t x[2][G][2], p[2][G];
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++) {
+        const int tok = hf * 8 + (lane >> 2);
+        if constexpr (D == 64) {
+            const uint2 u = *reinterpret_cast<const uint2*>(gran + kv4_key_word<D>(tok, 0, 2 * t));
+            x[hf][0][0] = u.x, x[hf][0][1] = u.y;
+        } else {
+#pragma unroll
+            for (int gr = 0; gr < G; gr += 2) {
+                const uint4 u = *reinterpret_cast<const uint4*>(gran + kv4_key_word<D>(tok, gr, 2 * t));
+                x[hf][gr][0] = u.x, x[hf][gr][1] = u.y, x[hf][gr + 1][0] = u.z, x[hf][gr + 1][1] = u.w;
+            }
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; gr++) {
+            p[hf][gr] = *reinterpret_cast<const uint32_t*>(gran + kv4_kpar_off(D) + (tok * G + gr) * 4);
+            if (tok >= live) p[hf][gr] = 0u;
+        }
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+        for (int gr = 0; gr < G; gr++) {
+            const __half2 s2 = as_half2(dup_lo(p[hf][gr])), m2 = as_half2(dup_hi(p[hf][gr]));
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<uint4*>(out + gr * L::SUB + sw128_offset(row0 + hf * 8 + (lane >> 2), (2 * t + i) * 8)) =
+                    widen8(x[hf][gr][i], s2, m2);
+        }
+}
+
+// The values of a granule (`gran`: the granule's start, of which only the values' half is there).  NaN
+// groups become 0 (a key some row does not see must not reach it) and are named in bad[group] for the rows
+// that do see them; the writer gives both parameters NaN or neither.  Lanes: word lane % 8 of every group of
+// one token, four tokens at a time.
+template <int D>
+__device__ __forceinline__ void widen_values(const uint8_t* gran, int live, int row0, uint8_t* out, uint16_t* bad) {
+    using L = TileLayout<D>;
+    constexpr int G = L::G;
+    const int lane = threadIdx.x & 31, pc = lane & 7;
+    uint32_t x[4][G], p[4][G], nan[G];
+#pragma unroll
+    for (int gr = 0; gr < G; gr++)
+        nan[gr] = *reinterpret_cast<const uint32_t*>(gran + kv4_vpar_off(D) + ((lane & 15) * G + gr) * 4);
+#pragma unroll
+    for (int q4 = 0; q4 < 4; q4++) {
+        const int tok = q4 * 4 + (lane >> 3);
+        const uint8_t* src = gran + kv4_value_word<D>(tok, 0, pc);
+        if constexpr (D == 64) {
+            x[q4][0] = *reinterpret_cast<const uint32_t*>(src);
+        } else if constexpr (D == 128) {
+            const uint2 u = *reinterpret_cast<const uint2*>(src);
+            x[q4][0] = u.x, x[q4][1] = u.y;
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(src);
+            x[q4][0] = u.x, x[q4][1] = u.y, x[q4][2] = u.z, x[q4][3] = u.w;
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; gr++) {
+            p[q4][gr] = *reinterpret_cast<const uint32_t*>(gran + kv4_vpar_off(D) + (tok * G + gr) * 4);
+            if (tok >= live) p[q4][gr] = 0u;
+        }
+    }
+    uint32_t any = 0;
+#pragma unroll
+    for (int gr = 0; gr < G; gr++) {
+        nan[gr] = __ballot_sync(0xffffffffu, (lane & 15) < live && (nan[gr] & 0x7c00u) == 0x7c00u) & 0xffffu;
+        if (lane == 0) bad[gr * L::NG] = (uint16_t)nan[gr];
+        any |= nan[gr];
+    }
+    if (any) {
+#pragma unroll
+        for (int q4 = 0; q4 < 4; q4++)
+#pragma unroll
+            for (int gr = 0; gr < G; gr++)
+                if ((p[q4][gr] & 0x7c00u) == 0x7c00u) p[q4][gr] = 0u;
+    }
+#pragma unroll
+    for (int q4 = 0; q4 < 4; q4++)
+#pragma unroll
+        for (int gr = 0; gr < G; gr++)
+            *reinterpret_cast<uint4*>(out + gr * L::SUB + sw128_offset(row0 + q4 * 4 + (lane >> 3), pc * 8)) =
+                widen8(x[q4][gr], as_half2(dup_lo(p[q4][gr])), as_half2(dup_hi(p[q4][gr])));
+}
+
 template <int D>
 __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4AttnArgs a) {
     using L = TileLayout<D>;
-    constexpr int G = L::G, MT = L::MT, NK = L::NK;
+    constexpr int G = L::G, MT = L::MT, NK = L::NK, NG = L::NG;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_slot;
-    __shared__ int red[L::THREADS / 32], pick[2];
+    __shared__ int red[L::THREADS / 32], pick[5], few[kTlFew];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + L::BAR);  // [deq warps][RING]
-    uint64_t* kfull = raw_full + kTlDeqWarps * L::RING;
+    uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + L::BAR);  // [widening warps][RING]
+    uint64_t* kfull = raw_full + L::WIDEN * L::RING;
     uint64_t* kempty = kfull + L::KST;
     uint64_t* vfull = kempty + L::KST;
     uint64_t* vempty = vfull + L::VST;
@@ -171,9 +293,9 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     uint64_t* odone = pfull + 2;        // [2] (MT = 1: the first)
     uint64_t* qfull = odone + 2;
     if (tid == 0) {
-        for (int i = 0; i < kTlDeqWarps * L::RING; i++) mbar_init(&raw_full[i], 1);
-        for (int i = 0; i < L::KST; i++) mbar_init(&kfull[i], kTlDeqWarps), mbar_init(&kempty[i], 1);
-        for (int i = 0; i < L::VST; i++) mbar_init(&vfull[i], kTlDeqWarps), mbar_init(&vempty[i], 1);
+        for (int i = 0; i < L::WIDEN * L::RING; i++) mbar_init(&raw_full[i], 1);
+        for (int i = 0; i < L::KST; i++) mbar_init(&kfull[i], NG), mbar_init(&kempty[i], 1);
+        for (int i = 0; i < L::VST; i++) mbar_init(&vfull[i], NG), mbar_init(&vempty[i], 1);
         for (int i = 0; i < 2; i++) mbar_init(&sfull[i], 1), mbar_init(&pfull[i], 4), mbar_init(&odone[i], 1);
         mbar_init(qfull, L::SM_WARPS);
         fence_mbar_init();
@@ -182,26 +304,17 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     // ---------------- the list's length; rows of blocks that see no key are zeroed here
     const size_t head_row = (size_t)a.heads * D;
     pdl_release();
-    auto steps = [&](int b) {
-        const Kv4Request r = kv4_request(a, b);
-        const int blocks = tile_blocks<D>(a, r);
-        int n = 0;
-        for (int u = 0; u < blocks; u++) {
-            const TileUnit t = tile_unit<D>(a, r, u);
-            n += t.n;
-            if (t.n == 0 && (b + u) % (int)gridDim.x == (int)blockIdx.x)
-                for (int h = 0; h < a.kv_heads; h++)
-                    for (int e = t.e0; e < t.e0 + t.rows; e++) {
-                        uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + e / a.group) * head_row +
-                                                            (size_t)(h * a.group + e % a.group) * D);
-                        for (int i = 0; i < D / 8; i++) o[i] = make_uint4(0, 0, 0, 0);
-                    }
-        }
-        return n * a.kv_heads;
-    };
     constexpr int W = L::THREADS / 32;
     int n0;
-    const int total = list_total<W>(a.requests, red, n0, steps);
+    const int total = tile_list_total<D, W>(a, red, few, n0, [&](int b, const Kv4Request& r, const TileUnit& t, int u) {
+        if (t.n == 0 && (b + u) % (int)gridDim.x == (int)blockIdx.x)
+            for (int h = 0; h < a.kv_heads; h++)
+                for (int e = t.e0; e < t.e0 + t.rows; e++) {
+                    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + e / a.group) * head_row +
+                                                        (size_t)(h * a.group + e % a.group) * D);
+                    for (int i = 0; i < D / 8; i++) o[i] = make_uint4(0, 0, 0, 0);
+                }
+    });
     const RunCut run(total, gridDim.x);
     const int cta = blockIdx.x;
     if (total == 0 || cta >= run.ctas) {
@@ -210,8 +323,8 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     }
     const int start = run.start(cta);
     const int len = run.start(cta + 1) - start;  // this CTA's run
-    list_find<W>(a.requests, red, pick, n0, start, steps);
-    if (warp == L::SM_WARPS + kTlDeqWarps) {
+    tile_list_find<D, W>(a, red, pick, n0, start);
+    if (warp == L::MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -222,16 +335,18 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     const uint32_t tmem = tmem_slot;
     TileCursor cur;
     cur.b = pick[0];
-    cur.beg = pick[1] - start;
     tile_load<D>(a, cur);
+    cur.u = pick[2], cur.h = pick[4];
+    cur.beg = pick[3] - start;
+    cur.t = tile_unit<D>(a, cur.r, cur.u);
 
     if (warp < L::SM_WARPS) {
         // ---------------- softmax: one thread a (row, head) pair of row tile `mt`
         const int mt = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t o_tm = tmem + lanes + L::O_COL + mt * D;
-        uint32_t turns = 0;   // tiles this row tile has taken
-        uint32_t tiles = 0;   // tiles the CTA has taken (the value ring's turn)
+        uint32_t turns = 0;  // tiles this row tile has taken
+        uint32_t tiles = 0;  // tiles the CTA has taken (the key and value rings' turn)
         bool ok = true;
         for (int pos = 0; pos < len;) {
             // both row tiles start a unit together: one that sits a unit out must not count for the next
@@ -242,15 +357,14 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             const int seg_end = min(len, cur.beg + un.n);
             const int j0 = pos - cur.beg, n = seg_end - pos;
             const int e = mt * 128 + row;
-            const bool live = e < un.rows;                    // this thread has a pair
-            const bool tile_live = mt * 128 < un.rows;        // the row tile takes part
+            const bool live = e < un.rows;              // this thread has a pair
+            const bool tile_live = mt * 128 < un.rows;  // the row tile takes part
             const int pair = un.e0 + (live ? e : 0);
             const int qi = pair / a.group, head = cur.h * a.group + pair % a.group;
             const int qpos = r.pos0 + qi;
 
             // the query row: scaled by a power of two (largest entry to [2^13, 2^14)), F16, chunk order
             const long long at = (r.q0 + qi) * a.qts + head * a.qhs;
-            float top = 0.0f;
             auto load8q = [&](int c, float (&x)[8]) {
                 if (!live) {
 #pragma unroll
@@ -268,7 +382,8 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                     for (int i = 0; i < 8; i++) x[i] = load_act(a.q, (size_t)(at + c + i), a.dt);
                 }
             };
-#pragma unroll 4
+            float top = 0.0f;
+#pragma unroll 8
             for (int c = 0; c < D; c += 8) {
                 float x[8];
                 load8q(c, x);
@@ -279,8 +394,9 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             if (top > 0.0f && top < 3.0e38f) k2 = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -120), 120);
             // a negative scale goes into the query's sign, so that c >= 0 below
             const float up = copysignf(__uint_as_float((uint32_t)(k2 + 127) << 23), a.scale_log2);
-            const float c = fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k2) << 23);
-#pragma unroll 4
+            // (a scale of 0 keeps c above 0: -inf c is then -inf, and what is left of the scores adds nothing)
+            const float c = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k2) << 23), 1.0e-30f);
+#pragma unroll 8
             for (int ch = 0; ch < D; ch += 8) {
                 float x[8];
                 load8q(ch, x);
@@ -297,6 +413,10 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             __syncwarp();
             if (lane == 0) mbar_arrive(qfull);
 
+            const int lowest = a.window > 0 ? qpos - a.window + 1 : 0, highest = min(r.hi - 1, qpos);
+            // tiles of keys that start at or after full_lo and end by full_hi are seen whole by every pair
+            const int full_hi = min(r.hi, r.pos0 + un.e0 / a.group + 1) - NK;
+            const int full_lo = a.window > 0 ? r.pos0 + (un.e0 + un.rows - 1) / a.group - a.window + 1 : 0;
             float mref = -1.0e30f, l = 0.0f;
             uint32_t bad = 0;  // groups in which the row sees a NaN value
             for (int j = 0; tile_live && j < n; j++, turns++) {
@@ -306,67 +426,66 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                 const int k0 = un.lo + (j0 + j) * NK;
                 if (ok) ok = mbar_wait(&sfull[bi], par, DEV_TIMEOUT_FULL);
                 tc_fence_after();
-                // every key of the tile seen by every pair of the block (pages outside the pool aside)?
-                const int first = r.pos0 + un.e0 / a.group, last = r.pos0 + (un.e0 + un.rows - 1) / a.group;
-                bool full = k0 + NK <= min(r.hi, first + 1) && (a.window == 0 || k0 > last - a.window);
-                uint32_t gone = 0;  // 16-key granules without a page
-                const int lowest = a.window > 0 ? qpos - a.window + 1 : 0, highest = min(r.hi - 1, qpos);
+                bool full = k0 >= full_lo && k0 <= full_hi;
+                uint32_t gone = 0;  // granules without a page
                 {
-                    const uint32_t vt = tiles + j;
-                    if (ok) ok = mbar_wait(&vfull[vt % L::VST], (vt / L::VST) & 1, DEV_TIMEOUT_FULL);
-                    const uint32_t* bm = reinterpret_cast<const uint32_t*>(smem + L::BAD + (vt % L::VST) * (G * (NK / 16) * 2));
+                    const uint32_t* gm = reinterpret_cast<const uint32_t*>(smem + L::GONE + ((tiles + j) & 3) * NG);
                     uint32_t any = 0;
 #pragma unroll
-                    for (int i = 0; i < G * (NK / 32); i++) any |= bm[i];
+                    for (int i = 0; i < NG / 4; i++) any |= gm[i];
                     if (any) {
-                        // bit 16 i + t of a group: key 16 i + t holds NaN; both a granule without a page
-                        // (every bit of every group) and NaN values come this way
-                        for (int i = 0; i < NK / 16; i++) {
-                            uint32_t all = 0xffffu;
-                            for (int gr = 0; gr < G; gr++) all &= reinterpret_cast<const uint16_t*>(bm)[gr * (NK / 16) + i];
-                            const int key = k0 + 16 * i;
-                            const int pg = key < r.hi ? a.table[cur.b * a.tstride + (key >> a.shift)] : -1;
-                            if (all == 0xffffu && (pg < 0 || pg >= a.pages)) {
-                                gone |= 1u << i;
-                                continue;
-                            }
-                            for (int gr = 0; gr < G; gr++) {
-                                const uint32_t m = reinterpret_cast<const uint16_t*>(bm)[gr * (NK / 16) + i];
-                                for (int t = 0; t < 16; t++)
-                                    if (((m >> t) & 1u) && key + t >= lowest && key + t <= highest) bad |= 1u << gr;
-                            }
-                        }
-                        full = full && gone == 0;
+                        for (int i = 0; i < NG; i++) gone |= ((gm[i >> 2] >> (8 * (i & 3))) & 1u) << i;
+                        full = false;
                     }
                 }
-                auto masked = [&](int i) {  // key i of the tile
-                    const int key = k0 + i;
-                    return key < lowest || key > highest || ((gone >> (i >> 4)) & 1u);
-                };
-                float mx = -CUDART_INF_F;
+                if (!full) {
+                    // keys this row does not see score -inf from here on
 #pragma unroll 1
-                for (int q = 0; q < NK; q += 32) {
-                    float v[32];
-                    __syncwarp();
-                    tmem_ld32(s_tm + q, v);
-                    if (!full) {
+                    for (int q = 0; q < NK; q += 32) {
+                        const int from = max(lowest - k0 - q, 0), to = min(highest - k0 - q, 31);  // the row's keys among the 32
+                        uint32_t seen = from > 31 || to < from ? 0u : (0xffffffffu << from) & (0xffffffffu >> (31 - to));
+                        if ((gone >> (q >> 4)) & 1u) seen &= 0xffff0000u;
+                        if ((gone >> (q >> 4)) & 2u) seen &= 0x0000ffffu;
+                        uint32_t v[32];
+                        __syncwarp();
+                        tmem_ld32_start(s_tm + q, v);
+                        tmem_ld32_wait(v);
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (masked(q + i)) v[i] = -CUDART_INF_F;
+                        for (int i = 0; i < 32; i++) v[i] = (seen >> i) & 1u ? v[i] : 0xff800000u;
+                        tmem_st32u(s_tm + q, v);
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, v[i]);
+                    tmem_st_wait();
                 }
-                mx = mx == -CUDART_INF_F ? mx : mx * c;
+                float m4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+                uint32_t va[32], vb[32];
+                auto top_of = [&](uint32_t (&v)[32]) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(v[i]));
+                };
+                __syncwarp();
+                tmem_ld32_start(s_tm, va);
+#pragma unroll 1
+                for (int q = 0; q < NK; q += 64) {
+                    tmem_ld32_wait(va);
+                    tmem_ld32_start(s_tm + q + 32, vb);
+                    top_of(va);
+                    __syncwarp();
+                    tmem_ld32_wait(vb);
+                    tmem_ld32_start(s_tm + (q + 64 < NK ? q + 64 : 0), va);  // the last: the first for the second pass
+                    top_of(vb);
+                    __syncwarp();
+                }
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
                 if (__any_sync(0xffffffffu, mx > mref + 15.0f)) {
                     const float moved = fmaxf(mref, mx - 7.0f);
                     const float f = ex2(mref - moved);
                     mref = moved;
                     l *= f;
                     if (j > 0) {
-                        const uint32_t ot = turns - 1;  // the product of the tile before is in
-                        if (ok) ok = mbar_wait(&odone[MT == 2 ? mt : 0], ot & 1, DEV_TIMEOUT_FULL);
+                        // the product of the tile before is in
+                        if (ok) ok = mbar_wait(&odone[MT == 2 ? mt : 0], (turns - 1) & 1, DEV_TIMEOUT_FULL);
                         tc_fence_after();
+                        tmem_ld32_wait(va);
 #pragma unroll 1
                         for (int q = 0; q < D; q += 32) {
                             float v[32];
@@ -377,25 +496,47 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                         }
                     }
                 }
-#pragma unroll 1
-                for (int q = 0; q < NK; q += 32) {
-                    float v[32];
-                    tmem_ld32(s_tm + q, v);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = ex2(fmaf(v[i], c, -mref));
-                    if (!full) {
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            if (masked(q + i)) v[i] = 0.0f;
-                    }
-                    uint32_t w[16];
+                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                auto weights = [&](uint32_t (&v)[32], uint32_t* w) {
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        l += v[2 * i] + v[2 * i + 1];
-                        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                        const float p0 = ex2(fmaf(__uint_as_float(v[2 * i]), c, -mref));
+                        const float p1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), c, -mref));
+                        l4[i & 3] += p0 + p1;
+                        const __half2 h = __floats2half2_rn(p0, p1);
                         w[i] = *reinterpret_cast<const uint32_t*>(&h);
                     }
-                    tmem_st16(s_tm + q / 2, w);
+                };
+                // the weights of columns q go over columns q / 2, which are in registers by then; 64 at a
+                // time, since a store holds up the warp's later loads while the products run
+#pragma unroll 1
+                for (int q = 0; q < NK; q += 64) {
+                    uint32_t w[32];
+                    tmem_ld32_wait(va);
+                    tmem_ld32_start(s_tm + q + 32, vb);
+                    weights(va, w);
+                    __syncwarp();
+                    tmem_ld32_wait(vb);
+                    if (q + 64 < NK) tmem_ld32_start(s_tm + q + 64, va);
+                    weights(vb, w + 16);
+                    __syncwarp();
+                    tmem_st32u(s_tm + q / 2, w);
+                }
+                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                {
+                    // value groups with NaN (widened to 0): named for the rows that see them
+                    const uint32_t vt = tiles + j;
+                    if (ok) ok = mbar_wait(&vfull[vt % L::VST], (vt / L::VST) & 1, DEV_TIMEOUT_FULL);
+                    const uint32_t* bm = reinterpret_cast<const uint32_t*>(smem + L::BAD + (vt % L::VST) * (G * NG * 2));
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < G * NG / 2; i++) any |= bm[i];
+                    if (any)
+                        for (int i = 0; i < G * NK; i++) {
+                            const int key = k0 + i % NK;
+                            if (((bm[i >> 5] >> (i & 31)) & 1u) && key >= lowest && key <= highest) bad |= 1u << (i / NK);
+                        }
+                    __syncwarp();
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -406,7 +547,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
 
             // ---------------- the rows out, or this CTA's share of them into its slot
             const bool whole = j0 == 0 && n == un.n;
-            float* slot = a.part + (size_t)(2 * cta + (pos == 0 ? 0 : 1)) * (L::ROWS * (D + 2));
+            float* slot = a.part + (size_t)(2 * cta + (pos == 0 ? 0 : 1)) * (kv4_tile_rows(D) * (D + 2));
             if (tile_live) {
                 if (ok) ok = mbar_wait(&odone[MT == 2 ? mt : 0], (turns - 1) & 1, DEV_TIMEOUT_FULL);
                 tc_fence_after();
@@ -426,7 +567,8 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
 #pragma unroll
                             for (int i = 0; i < 8; i++) x[chunk_channel(i)] = v[w + i];
                             if (whole) {
-                                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + qi) * head_row + (size_t)head * D + q + w) =
+                                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + qi) * head_row +
+                                                          (size_t)head * D + q + w) =
                                     make_uint4(pack_act2(x[0], x[1], a.dt), pack_act2(x[2], x[3], a.dt),
                                                pack_act2(x[4], x[5], a.dt), pack_act2(x[6], x[7], a.dt));
                             } else {
@@ -440,137 +582,80 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                 __syncwarp();
                 tc_fence_before();  // the next unit's first product overwrites O after the next arrival
                 if (!whole && live)
-                    __stcg(reinterpret_cast<float2*>(slot + L::ROWS * D + 2 * e), make_float2(mref, l));
+                    __stcg(reinterpret_cast<float2*>(slot + kv4_tile_rows(D) * D + 2 * e), make_float2(mref, l));
             }
             pos = seg_end;
         }
-    } else if (warp < L::SM_WARPS + kTlDeqWarps) {
-        // ---------------- widening: warp w takes granules w GPW .. of every tile
+    } else if (warp < L::MMA_WARP) {
+        // ---------------- widening: task q of the run is granule q % NG of tile q / (2 NG), its keys, then its values
         const int w = warp - L::SM_WARPS;
-        uint8_t* ring = smem + L::RAW + w * L::RING * L::GB;
+        uint8_t* ring = smem + L::RAW + w * L::RING * L::HB;
         uint64_t* bar = raw_full + w * L::RING;
-        uint32_t tiles = 0, taken = 0;  // tiles widened, granules consumed
-        uint32_t there = 0;             // a bit a ring place: the granule was copied
+        uint32_t there = 0;  // a bit a ring place: the granule was copied
         bool ok = true;
-        for (int pos = 0; pos < len;) {
-            tile_seek<D>(a, cur, pos);
-            const Kv4Request r = cur.r;
-            const int seg_end = min(len, cur.beg + cur.t.n);
-            const int n = seg_end - pos;
-            const int lo = cur.t.lo + (pos - cur.beg) * NK;
-            auto issue = [&](int q) {  // granule q of the warp's share of the segment, into place (taken + q) % RING
-                const int key = lo + (q / L::GPW) * NK + (w * L::GPW + q % L::GPW) * kKvGranule;
-                const int place = (int)((taken + q) % L::RING);
-                int page = -1;
-                if (key < r.hi) page = a.table[cur.b * a.tstride + (key >> a.shift)];
-                const bool got = page >= 0 && page < a.pages;
+        TileCursor ahead = cur;
+        const int tasks = len * 2 * NG;
+        int in_q = w, in_place = 0;
+        // the next copy's place in the cache, looked up a copy ahead (its page id is a load of its own)
+        const uint8_t* next = nullptr;
+        int next_page = -1;
+        auto look = [&]() {
+            next_page = -1;
+            if (in_q >= tasks) return;
+            const int tile = in_q / (2 * NG), part = in_q % (2 * NG);
+            tile_seek<D>(a, ahead, tile);
+            const int key = ahead.t.lo + (tile - ahead.beg) * NK + (part % NG) * kKvGranule;
+            if (key < ahead.r.hi) next_page = a.table[ahead.b * a.tstride + (key >> a.shift)];
+            next = a.pool + (part >= NG ? kv4_value_off(D) : 0) +
+                   kv4_granule<D>(0, a.kv_heads, ahead.h, a.page_size, key & (a.page_size - 1));
+        };
+        const size_t page_bytes = kv4_granule<D>(1, a.kv_heads, 0, a.page_size, 0);
+        auto issue = [&]() {  // the warp's next copy into its next ring place
+            if (in_q < tasks) {
+                const bool got = next_page >= 0 && next_page < a.pages;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&bar[place], got ? L::GB : 0);
-                    if (got)
-                        bulk_g2s(ring + place * L::GB,
-                                 a.pool + kv4_granule<D>(page, a.kv_heads, cur.h, a.page_size, key & (a.page_size - 1)), L::GB,
-                                 &bar[place]);
+                    mbar_arrive_expect_tx(&bar[in_place], got ? L::HB : 0);
+                    if (got) bulk_g2s(ring + in_place * L::HB, next + next_page * page_bytes, L::HB, &bar[in_place]);
                 }
-                there = (there & ~(1u << place)) | ((got ? 1u : 0u) << place);
-            };
-            for (int q = 0; q < L::RING && q < n * L::GPW; q++) issue(q);
-            for (int j = 0; j < n; j++, tiles++) {
-                const int kb = tiles % L::KST, vb = tiles % L::VST;
-                const int k0 = lo + j * NK + w * L::GPW * kKvGranule;  // the warp's first key
-                if (ok && tiles >= (uint32_t)L::KST) ok = mbar_wait(&kempty[kb], (tiles / L::KST - 1) & 1, DEV_TIMEOUT_EMPTY);
-                uint8_t* kt = smem + L::K + kb * L::KV_TILE;
-#pragma unroll
-                for (int gi = 0; gi < L::GPW; gi++) {
-                    const uint32_t q = taken + j * L::GPW + gi;
-                    const int place = (int)(q % L::RING);
-                    if (ok) ok = mbar_wait(&bar[place], (q / L::RING) & 1, DEV_TIMEOUT_FULL);
-                    const uint8_t* gran = ring + place * L::GB;
-                    const bool got = (there >> place) & 1u;
-                    const int t = lane & 3;
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        const int tok = half * 8 + (lane >> 2);
-                        const bool seen = got && k0 + gi * kKvGranule + tok < r.hi;
-                        const int row = (w * L::GPW + gi) * kKvGranule + tok;
-                        uint32_t x[G][2];
-                        if constexpr (D == 64) {
-                            const uint2 u = *reinterpret_cast<const uint2*>(gran + kv4_key_word<D>(tok, 0, 2 * t));
-                            x[0][0] = u.x, x[0][1] = u.y;
-                        } else {
-#pragma unroll
-                            for (int gr = 0; gr < G; gr += 2) {
-                                const uint4 u = *reinterpret_cast<const uint4*>(gran + kv4_key_word<D>(tok, gr, 2 * t));
-                                x[gr][0] = u.x, x[gr][1] = u.y, x[gr + 1][0] = u.z, x[gr + 1][1] = u.w;
-                            }
-                        }
-#pragma unroll
-                        for (int gr = 0; gr < G; gr++) {
-                            const uint32_t p = seen ? *reinterpret_cast<const uint32_t*>(gran + kv4_kpar_off(D) + (tok * G + gr) * 4) : 0u;
-                            const __half2 s2 = as_half2(dup_lo(p)), m2 = as_half2(dup_hi(p));
-#pragma unroll
-                            for (int i = 0; i < 2; i++)
-                                *reinterpret_cast<uint4*>(kt + gr * L::SUB + sw128_offset(row, (2 * t + i) * 8)) = widen8(x[gr][i], s2, m2);
-                        }
-                    }
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&kfull[kb]);
-
-                if (ok && tiles >= (uint32_t)L::VST) ok = mbar_wait(&vempty[vb], (tiles / L::VST - 1) & 1, DEV_TIMEOUT_EMPTY);
-                uint8_t* vt = smem + L::V + vb * L::KV_TILE;
-                uint16_t* bm = reinterpret_cast<uint16_t*>(smem + L::BAD) + vb * (G * (NK / 16));
-#pragma unroll
-                for (int gi = 0; gi < L::GPW; gi++) {
-                    const int place = (int)((taken + j * L::GPW + gi) % L::RING);
-                    const uint8_t* gran = ring + place * L::GB;
-                    const bool got = (there >> place) & 1u;
-                    const int kg = k0 + gi * kKvGranule;
-                    // NaN groups are widened to 0 (a key some row does not see must not reach it) and
-                    // named for the rows that do see them; so is a granule without a page
-#pragma unroll
-                    for (int gr = 0; gr < G; gr++) {
-                        const uint32_t p = *reinterpret_cast<const uint32_t*>(gran + kv4_vpar_off(D) + ((lane & 15) * G + gr) * 4);
-                        const bool nan = !got ? kg < r.hi : (kg + (lane & 15) < r.hi && ((p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u));
-                        const uint32_t m = __ballot_sync(0xffffffffu, nan) & 0xffffu;
-                        if (lane == 0) bm[gr * (NK / 16) + w * L::GPW + gi] = (uint16_t)m;
-                    }
-                    // lanes: piece pc of a row (D / 8 words in 8 pieces), four tokens at a time
-                    const int pc = lane & 7;
-#pragma unroll
-                    for (int q4 = 0; q4 < 4; q4++) {
-                        const int tok = q4 * 4 + (lane >> 3);
-                        const bool seen = got && kg + tok < r.hi;
-                        const int row = (w * L::GPW + gi) * kKvGranule + tok;
-                        const uint8_t* src = gran + kv4_value_word<D>(tok, 0, pc);
-                        uint32_t x[G];
-                        if constexpr (D == 64) {
-                            x[0] = *reinterpret_cast<const uint32_t*>(src);
-                        } else if constexpr (D == 128) {
-                            const uint2 u = *reinterpret_cast<const uint2*>(src);
-                            x[0] = u.x, x[1] = u.y;
-                        } else {
-                            const uint4 u = *reinterpret_cast<const uint4*>(src);
-                            x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-                        }
-#pragma unroll
-                        for (int gr = 0; gr < G; gr++) {
-                            uint32_t p = seen ? *reinterpret_cast<const uint32_t*>(gran + kv4_vpar_off(D) + (tok * G + gr) * 4) : 0u;
-                            if ((p & 0x7c00u) == 0x7c00u || (p & 0x7c000000u) == 0x7c000000u) p = 0u;
-                            *reinterpret_cast<uint4*>(vt + gr * L::SUB + sw128_offset(row, pc * 8)) =
-                                widen8(x[gr], as_half2(dup_lo(p)), as_half2(dup_hi(p)));
-                        }
-                    }
-                    __syncwarp();
-                    const int q = j * L::GPW + gi + L::RING;
-                    if (q < n * L::GPW) issue(q);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&vfull[vb]);
+                there = (there & ~(1u << in_place)) | ((got ? 1u : 0u) << in_place);
             }
-            taken += n * L::GPW;
-            pos = seg_end;
+            in_q += L::WIDEN;
+            if (++in_place == L::RING) in_place = 0;
+            look();
+        };
+        look();
+        for (int i = 0; i < L::RING; i++) issue();
+        int place = 0;
+        uint32_t parity = 0;
+        for (int task = w; task < tasks; task += L::WIDEN) {
+            const uint32_t tile = task / (2 * NG);
+            const int part = task % (2 * NG), gi = part % NG;
+            tile_seek<D>(a, cur, (int)tile);
+            const int first = cur.t.lo + ((int)tile - cur.beg) * NK + gi * kKvGranule;  // the granule's first key
+            const bool got = (there >> place) & 1u;
+            const int live = got ? min(cur.r.hi - first, kKvGranule) : 0;  // tokens that are there
+            const uint8_t* raw = ring + place * L::HB;
+            uint64_t* full;
+            if (part < NG) {
+                const int stage = (int)(tile % L::KST);
+                full = &kfull[stage];
+                if (ok && tile >= L::KST) ok = mbar_wait(&kempty[stage], (tile / L::KST - 1) & 1, DEV_TIMEOUT_EMPTY);
+                if (ok) ok = mbar_wait(&bar[place], parity, DEV_TIMEOUT_FULL);
+                if (lane == 0) smem[L::GONE + (tile & 3) * NG + gi] = !got && first < cur.r.hi;
+                widen_keys<D>(raw, live, gi * kKvGranule, smem + L::K + stage * L::KV_TILE);
+            } else {
+                const int stage = (int)(tile % L::VST);
+                full = &vfull[stage];
+                if (ok && tile >= L::VST) ok = mbar_wait(&vempty[stage], (tile / L::VST - 1) & 1, DEV_TIMEOUT_EMPTY);
+                if (ok) ok = mbar_wait(&bar[place], parity, DEV_TIMEOUT_FULL);
+                widen_values<D>(raw - kv4_value_off(D), live, gi * kKvGranule, smem + L::V + stage * L::KV_TILE,
+                                reinterpret_cast<uint16_t*>(smem + L::BAD) + stage * (G * NG) + gi);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+            issue();
+            if (++place == L::RING) place = 0, parity ^= 1u;
         }
     } else if (lane == 0) {
         // ---------------- the products
@@ -644,7 +729,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     pdl_wait();  // the join that follows waits for this grid: the streaming kernel's end is part of it
     tc_fence_before();
     __syncthreads();
-    if (warp == L::SM_WARPS + kTlDeqWarps) {
+    if (warp == L::MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
