@@ -122,20 +122,25 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(
 }
 
 // ------------------------------------------------------------------ write and read
-// A thread takes eight consecutive channels of a token's key or value: one 16-byte load (16-bit
-// types), the group's minimum and maximum over its eight lanes by shuffles, one 32-bit word of codes.
-// Both kernels are HBM bound, one pass over the data.
+// A thread takes eight consecutive channels of a token's key AND value: two 16-byte loads in flight
+// (16-bit types), each group's minimum and maximum over its eight lanes by shuffles, one 32-bit word of
+// codes each.  Both kernels are HBM bound, one pass over the data.  The grid's y walks the tokens, so an
+// item's head and piece come from 32-bit arithmetic (a 64-bit division an item took most of the time:
+// 8192 tokens of 8 heads of 128, written and read back, 76 us with it).
 constexpr int kKvThreads = 256;
+constexpr int kKvMostHeads = 65536;  // a token's items, and a CTA's, stay in 32 bits
 
 struct KvIoArgs {
     uint8_t* pool;
     long long places;  // pages * page_size
     int kv_heads, page_size, shift;
+    int row_items;  // kv_heads * D / 8: a token's items
     const void* src[2];  // write: k, v
     long long ts[2], hs[2];
     void* dst[2];  // read: k, v
     const long long* slots;
     int tokens;
+    int per_cta;  // tokens a CTA
     int dt;
     int vec;  // every row of eight channels starts 16-byte aligned
 };
@@ -161,24 +166,8 @@ __device__ __forceinline__ void load8(const void* p, long long i, int dt, bool v
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kKvThreads) kv4_write_kernel(KvIoArgs a) {
-    constexpr int W = D / 8;  // words of a row
-    const long long item = (long long)blockIdx.x * kKvThreads + threadIdx.x;
-    const long long row = item / W;  // (token, key or value, head)
-    const int piece = (int)(item % W);
-    const int h = (int)(row % a.kv_heads);
-    const int kv = (int)((row / a.kv_heads) & 1);
-    const long long t = row / a.kv_heads / 2;
-    // The eight lanes of a group share a token, so they leave together and the shuffles below name
-    // only lanes that are there.
-    if (t >= a.tokens) return;
-    const long long slot = a.slots[t];
-    if (slot < 0 || slot >= a.places) return;
-    const unsigned lanes = 0xffu << (threadIdx.x & 24);
-
-    float x[8];
-    load8(a.src[kv], t * a.ts[kv] + h * a.hs[kv] + piece * 8, a.dt, a.vec, x);
+// A group's codes and parameters; the eight lanes of `lanes` hold its 64 channels, eight each.
+__device__ __forceinline__ uint32_t encode8(float (&x)[8], unsigned lanes, uint32_t& par) {
     bool bad = false;
     float lo = kKvLargest, hi = -kKvLargest;
 #pragma unroll
@@ -212,58 +201,92 @@ __global__ void __launch_bounds__(kKvThreads) kv4_write_kernel(KvIoArgs a) {
             word |= (uint32_t)min(max(__float2int_rn(q), 0), 15) << (4 * j);
         }
     }
-    const int tok = (int)(slot & (a.page_size - 1));
-    uint8_t* gran = a.pool + kv4_granule<D>(slot >> a.shift, a.kv_heads, h, a.page_size, tok);
-    const int gt = tok & (kKvGranule - 1), gr = piece >> 3, w = piece & 7;
-    *reinterpret_cast<uint32_t*>(gran + (kv ? kv4_value_word<D>(gt, gr, w) : kv4_key_word<D>(gt, gr, w))) = word;
-    if (w == 0)
-        *reinterpret_cast<uint32_t*>(gran + (kv ? kv4_vpar_off(D) : kv4_kpar_off(D)) + (gt * (D / kKvGroup) + gr) * 4) =
-            (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mh) << 16);
+    par = (uint32_t)__half_as_ushort(sh) | ((uint32_t)__half_as_ushort(mh) << 16);
+    return word;
+}
+
+// Item i of a CTA's tokens [t0, t0 + n): token, head and piece.
+struct KvItem {
+    int t, h, piece;
+};
+template <int D>
+__device__ __forceinline__ KvItem kv_item(const KvIoArgs& a, int t0, int i) {
+    const unsigned t = (unsigned)i / (unsigned)a.row_items, rest = i - t * a.row_items;
+    return {t0 + (int)t, (int)(rest / (D / 8)), (int)(rest % (D / 8))};
+}
+
+template <int D>
+__global__ void __launch_bounds__(kKvThreads) kv4_write_kernel(KvIoArgs a) {
+    const int t0 = blockIdx.x * a.per_cta;
+    const int items = min(a.per_cta, a.tokens - t0) * a.row_items;
+    const unsigned lanes = 0xffu << (threadIdx.x & 24);
+    // The eight lanes of a group share a token and head, so they leave and skip together and the shuffles
+    // name only lanes that are there.
+    for (int i = blockIdx.y * kKvThreads + threadIdx.x; i < items; i += gridDim.y * kKvThreads) {
+        const KvItem it = kv_item<D>(a, t0, i);
+        const long long slot = a.slots[it.t];
+        if (slot < 0 || slot >= a.places) continue;
+        float k[8], v[8];
+        load8(a.src[0], it.t * a.ts[0] + it.h * a.hs[0] + it.piece * 8, a.dt, a.vec, k);
+        load8(a.src[1], it.t * a.ts[1] + it.h * a.hs[1] + it.piece * 8, a.dt, a.vec, v);
+        uint32_t kp, vp;
+        const uint32_t kw = encode8(k, lanes, kp), vw = encode8(v, lanes, vp);
+        const int tok = (int)(slot & (a.page_size - 1));
+        uint8_t* gran = a.pool + kv4_granule<D>(slot >> a.shift, a.kv_heads, it.h, a.page_size, tok);
+        const int gt = tok & (kKvGranule - 1), gr = it.piece >> 3, w = it.piece & 7;
+        *reinterpret_cast<uint32_t*>(gran + kv4_key_word<D>(gt, gr, w)) = kw;
+        *reinterpret_cast<uint32_t*>(gran + kv4_value_word<D>(gt, gr, w)) = vw;
+        if (w == 0) *reinterpret_cast<uint32_t*>(gran + kv4_kpar_off(D) + (gt * (D / kKvGroup) + gr) * 4) = kp;
+        if (w == 1) *reinterpret_cast<uint32_t*>(gran + kv4_vpar_off(D) + (gt * (D / kKvGroup) + gr) * 4) = vp;
+    }
+}
+
+__device__ __forceinline__ void store8(void* p, long long o, int dt, bool vec, const float (&x)[8]) {
+    if (!vec) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) store_act(p, (size_t)(o + j), dt, x[j]);
+    } else if (dt == 0) {
+        float4* y = reinterpret_cast<float4*>(static_cast<float*>(p) + o);
+        y[0] = make_float4(x[0], x[1], x[2], x[3]);
+        y[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint16_t e0 = dt == 1 ? f2h(x[2 * j]) : __bfloat16_as_ushort(__float2bfloat16_rn(x[2 * j]));
+            const uint16_t e1 = dt == 1 ? f2h(x[2 * j + 1]) : __bfloat16_as_ushort(__float2bfloat16_rn(x[2 * j + 1]));
+            w[j] = (uint32_t)e0 | ((uint32_t)e1 << 16);
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + o) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 template <int D>
 __global__ void __launch_bounds__(kKvThreads) kv4_read_kernel(KvIoArgs a) {
-    constexpr int W = D / 8;
-    const long long item = (long long)blockIdx.x * kKvThreads + threadIdx.x;
-    const long long row = item / W;
-    const int piece = (int)(item % W);
-    const int h = (int)(row % a.kv_heads);
-    const int kv = (int)((row / a.kv_heads) & 1);
-    const long long t = row / a.kv_heads / 2;
-    if (t >= a.tokens) return;
-    const long long slot = a.slots[t];
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = 0.0f;
-    if (slot >= 0 && slot < a.places) {
-        const int tok = (int)(slot & (a.page_size - 1));
-        const uint8_t* gran = a.pool + kv4_granule<D>(slot >> a.shift, a.kv_heads, h, a.page_size, tok);
-        const int gt = tok & (kKvGranule - 1), gr = piece >> 3, w = piece & 7;
-        const uint32_t word =
-            *reinterpret_cast<const uint32_t*>(gran + (kv ? kv4_value_word<D>(gt, gr, w) : kv4_key_word<D>(gt, gr, w)));
-        const uint32_t par = *reinterpret_cast<const uint32_t*>(gran + (kv ? kv4_vpar_off(D) : kv4_kpar_off(D)) +
-                                                                (gt * (D / kKvGroup) + gr) * 4);
-        const float s = h2f((uint16_t)par), m = h2f((uint16_t)(par >> 16));
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = fmaf((float)((word >> (4 * j)) & 15u), s, m);
-    }
-    const long long o = (t * a.kv_heads + h) * D + piece * 8;
-    if (!a.vec) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) store_act(a.dst[kv], (size_t)(o + j), a.dt, x[j]);
-    } else if (a.dt == 0) {
-        float4* y = reinterpret_cast<float4*>(static_cast<float*>(a.dst[kv]) + o);
-        y[0] = make_float4(x[0], x[1], x[2], x[3]);
-        y[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        uint32_t p[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint16_t e0 = a.dt == 1 ? f2h(x[2 * j]) : __bfloat16_as_ushort(__float2bfloat16_rn(x[2 * j]));
-            const uint16_t e1 = a.dt == 1 ? f2h(x[2 * j + 1]) : __bfloat16_as_ushort(__float2bfloat16_rn(x[2 * j + 1]));
-            p[j] = (uint32_t)e0 | ((uint32_t)e1 << 16);
+    const int t0 = blockIdx.x * a.per_cta;
+    const int items = min(a.per_cta, a.tokens - t0) * a.row_items;
+    for (int i = blockIdx.y * kKvThreads + threadIdx.x; i < items; i += gridDim.y * kKvThreads) {
+        const KvItem it = kv_item<D>(a, t0, i);
+        const long long slot = a.slots[it.t];
+        uint32_t word[2] = {0, 0}, par[2] = {0, 0};  // 0 0: a place outside the pool reads 0
+        if (slot >= 0 && slot < a.places) {
+            const int tok = (int)(slot & (a.page_size - 1));
+            const uint8_t* gran = a.pool + kv4_granule<D>(slot >> a.shift, a.kv_heads, it.h, a.page_size, tok);
+            const int gt = tok & (kKvGranule - 1), gr = it.piece >> 3, w = it.piece & 7;
+            word[0] = *reinterpret_cast<const uint32_t*>(gran + kv4_key_word<D>(gt, gr, w));
+            word[1] = *reinterpret_cast<const uint32_t*>(gran + kv4_value_word<D>(gt, gr, w));
+            par[0] = *reinterpret_cast<const uint32_t*>(gran + kv4_kpar_off(D) + (gt * (D / kKvGroup) + gr) * 4);
+            par[1] = *reinterpret_cast<const uint32_t*>(gran + kv4_vpar_off(D) + (gt * (D / kKvGroup) + gr) * 4);
         }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dst[kv]) + o) = make_uint4(p[0], p[1], p[2], p[3]);
+        const long long o = ((long long)it.t * a.kv_heads + it.h) * D + it.piece * 8;
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+            const float s = h2f((uint16_t)par[kv]), m = h2f((uint16_t)(par[kv] >> 16));
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = fmaf((float)((word[kv] >> (4 * j)) & 15u), s, m);
+            store8(a.dst[kv], o, a.dt, a.vec, x);
+        }
     }
 }
 
@@ -289,14 +312,19 @@ KvIoArgs io_args(const sx_kv4* c, const int64_t* slots, int32_t tokens, sx_dtype
     a.slots = reinterpret_cast<const long long*>(slots);
     a.tokens = tokens;
     a.dt = dtype;
+    a.row_items = c->kv_heads * (c->head_dim / 8);
     return a;
 }
 
-// CTAs for one thread a word of keys and values; 0 when that passes a grid's 2^31 - 1.
-unsigned io_grid(const sx_kv4* c, int32_t tokens) {
-    const long long items = (long long)tokens * 2 * c->kv_heads * (c->head_dim / 8);
-    const long long ctas = (items + kKvThreads - 1) / kKvThreads;
-    return ctas > INT_MAX ? 0 : (unsigned)ctas;
+// The launch of one thread an item.  x: tokens, as many a CTA as make about 1024 items (long rows are
+// spread over y instead).
+dim3 io_grid(KvIoArgs& a) {
+    a.per_cta = std::max(1, 4 * kKvThreads / a.row_items);
+    const int y = std::min(std::max(1, a.row_items / (4 * kKvThreads)), 64);
+    // few tokens: one pass a thread
+    const int ctas = (a.tokens + a.per_cta - 1) / a.per_cta;
+    const int passes = (a.per_cta * a.row_items / y + kKvThreads - 1) / kKvThreads;
+    return dim3(ctas, std::min(64, ctas * y < 2 * sm_count() ? y * passes : y));
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -341,12 +369,11 @@ sx_status sx_kv4_write(sx_stream stream, const sx_kv4* cache, const void* k, int
     sx_status st = kv4_check(cache);
     if (st) return st;
     if (!dtype_ok(dtype)) return SX_ERR_BAD_DTYPE;
-    if (tokens < 0) return SX_ERR_BAD_SHAPE;
+    if (tokens < 0 || cache->kv_heads > kKvMostHeads) return SX_ERR_BAD_SHAPE;
     if (tokens == 0) return SX_OK;
     if (!k || !v || !slots) return SX_ERR_NULL_POINTER;
-    const unsigned grid = io_grid(cache, tokens);
-    if (!grid) return SX_ERR_BAD_SHAPE;
     KvIoArgs a = io_args(cache, slots, tokens, dtype);
+    const dim3 grid = io_grid(a);
     const int esz = dtype == SX_DT_F32 ? 4 : 2;
     a.src[0] = k, a.src[1] = v;
     a.ts[0] = k_token_stride, a.ts[1] = v_token_stride;
@@ -365,12 +392,11 @@ sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slot
     sx_status st = kv4_check(cache);
     if (st) return st;
     if (!dtype_ok(dtype)) return SX_ERR_BAD_DTYPE;
-    if (tokens < 0) return SX_ERR_BAD_SHAPE;
+    if (tokens < 0 || cache->kv_heads > kKvMostHeads) return SX_ERR_BAD_SHAPE;
     if (tokens == 0) return SX_OK;
     if (!k || !v || !slots) return SX_ERR_NULL_POINTER;
-    const unsigned grid = io_grid(cache, tokens);
-    if (!grid) return SX_ERR_BAD_SHAPE;
     KvIoArgs a = io_args(cache, slots, tokens, dtype);
+    const dim3 grid = io_grid(a);
     a.dst[0] = k, a.dst[1] = v;
     a.vec = aligned16(k) && aligned16(v);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
