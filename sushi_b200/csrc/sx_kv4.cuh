@@ -58,6 +58,8 @@ __device__ __forceinline__ size_t kv4_granule(long long page, int kv_heads, int 
            (size_t)(tok / kKvGranule) * kv4_granule_bytes(D);
 }
 
+constexpr int kKvMostRequests = 16384;  // a call's: two words each in shared memory
+
 inline bool kv4_page_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128 || p == 256; }
 inline bool kv4_dim_ok(int d) { return d == 64 || d == 128 || d == 256; }
 

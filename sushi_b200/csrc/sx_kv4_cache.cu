@@ -17,7 +17,6 @@ namespace sx {
 // table entry another CTA writes.  Bound by launch and load latency.
 constexpr int kTablesThreads = 256;
 constexpr int kTablesItems = 4;           // tokens a thread
-constexpr int kTablesMaxRequests = 16384;  // two sums of 4 bytes each in shared memory
 
 __device__ __forceinline__ int kv4_pages_of(int tokens, int shift) {
     return (int)(((unsigned)tokens + (1u << shift) - 1) >> shift);
@@ -345,7 +344,7 @@ sx_status sx_block_tables(sx_stream stream, const int32_t* ctx_lens, const int32
     if (!ctx_lens || !new_lens || !table || !free_pages || !free_count || !kv_lens || !cu_q || !free_left)
         return SX_ERR_NULL_POINTER;
     if (tokens > 0 && (!slots || !positions)) return SX_ERR_NULL_POINTER;
-    if (requests < 1 || requests > kTablesMaxRequests || !kv4_page_ok(page_size) || table_width < 1 ||
+    if (requests < 1 || requests > kKvMostRequests || !kv4_page_ok(page_size) || table_width < 1 ||
         table_stride < table_width || tokens < 0)
         return SX_ERR_BAD_SHAPE;
     const int smem = 2 * (requests + 1) * (int)sizeof(int);

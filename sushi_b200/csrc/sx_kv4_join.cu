@@ -1,12 +1,13 @@
 // The join of attention units that several CTAs shared: out = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k
 // over the shares k in CTA order, M = max m_k.
 //
-// Every place where the list of steps is cut gets CTAs of its own here (the first cut inside a unit
-// joins it, the unit's other cuts and cuts between units have nothing to do).  They find their unit
-// while the attention kernels still run (programmatic dependent launch) and wait only before reading the
-// shares, so what is left after the last attention CTA is a few dependent loads: for one request of 131071
-// keys and 8 key heads (55 shares a head) the in-kernel join by the last CTA to arrive took 12 us of
-// fence, counter and one SM's loads.  Bound by load latency.
+// The first cut of a kernel's list inside a unit stands for the unit's join; its other cuts, and cuts
+// between units, have nothing to do.  Everything but the shares themselves is known while the attention
+// kernels still run (programmatic dependent launch), so the units are found first and what is left after the
+// last attention CTA is two dependent loads: for one request of 131071 keys and 8 key heads (55 shares a
+// head) a join inside the attention kernel by the last CTA to arrive took 12 us of fence, counter and one
+// SM's loads.  Streaming kernel: a warp takes one column of a unit.  Tile kernel: a CTA takes 64 rows.
+// Bound by load latency.
 #include <cuda_runtime.h>
 
 #include "sx_kv4_attn.cuh"
@@ -18,44 +19,157 @@ constexpr int kJoinThreads = kJoinWarps * 32;
 constexpr int kJoinRows = 64;    // rows of a unit a CTA joins
 constexpr int kJoinShares = 64;  // shares whose weights are held at a time
 
+// One column of a unit the streaming kernel's CTAs shared, by one warp, or by `parts` warps of a group that
+// take the shares in turn and add up in `sums` (parts > 1; the group's barrier id).
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, Kv4AttnArgs ta, int stream_grid, int tile_grid) {
+__device__ __forceinline__ void join_column(const Kv4AttnArgs& a, const Kv4Request& r, int h, int c, const float* s0,
+                                            const float* s1, int shares, int part, int parts, float* sums, int barrier) {
+    constexpr int E = D / 32;  // channels a lane
+    constexpr size_t STRIDE = (size_t)kStRows * (D + 2);
+    const int lane = threadIdx.x & 31;
+    auto share = [&](int k) { return k == 0 ? s0 : s1 + (size_t)(2 * k) * STRIDE; };
+    // J shares' values and references are asked for before anything is worked out
+    constexpr int J = 64 / E < 16 ? 64 / E : 16;
+    float y[J][E], mw;
+    auto fetch = [&](int k0) {
+        mw = lane < J && k0 + lane * parts < shares ? __ldcg(share(k0 + lane * parts) + kStRows * D + 2 * c) : -1.0e30f;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+#pragma unroll
+            for (int e = 0; e < E; e++) y[j][e] = 0.0f;
+            if (k0 + j * parts < shares) {
+                const float* p = share(k0 + j * parts) + c * D + lane * E;
+                if constexpr (E == 2) {
+                    const float2 t = __ldcg(reinterpret_cast<const float2*>(p));
+                    y[j][0] = t.x, y[j][1] = t.y;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        const float4 t = __ldcg(reinterpret_cast<const float4*>(p + e));
+                        y[j][e] = t.x, y[j][e + 1] = t.y, y[j][e + 2] = t.z, y[j][e + 3] = t.w;
+                    }
+                }
+            }
+        }
+    };
+    fetch(part);
+    float top = -1.0e30f, ls = 0.0f;
+#pragma unroll 2
+    for (int k = lane; k < shares; k += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(share(k) + kStRows * D + 2 * c));
+        const float up = fmaxf(top, ml.x);
+        ls = fmaf(ls, ex2(top - up), ml.y * ex2(ml.x - up));
+        top = up;
+    }
+    float all = top;
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, m));
+    ls *= ex2(top - all);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, m);
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = 0.0f;
+    for (int k0 = part; k0 < shares;) {
+        const float w = ex2(mw - all);
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const float f = __shfl_sync(0xffffffffu, w, j);
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = k0 + j * parts < shares ? fmaf(f, y[j][e], v[e]) : v[e];
+        }
+        k0 += J * parts;
+        if (k0 < shares) fetch(k0);
+    }
+    if (parts > 1) {
+        if (part > 0) {
+#pragma unroll
+            for (int e = 0; e < E; e++) sums[part * D + lane * E + e] = v[e];
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(parts * 32) : "memory");
+        if (part == 0)
+            for (int p = 1; p < parts; p++)
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] += sums[p * D + lane * E + e];
+        asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(parts * 32) : "memory");
+        if (part > 0) return;
+    }
+    const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) +
+                                              ((size_t)(r.q0 + c / a.group) * a.heads + h * a.group + c % a.group) * D + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) o[e / 2] = pack_act2(v[e] * inv, v[e + 1] * inv, a.dt);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, Kv4AttnArgs ta, int stream_grid, int tile_grid,
+                                                                int stream_blocks) {
+    extern __shared__ int starts[];  // [requests + 1] the first step of each request in the streaming kernel's list
     __shared__ int red[kJoinWarps], pick[5], few[kTlFew];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool tile = (int)blockIdx.x >= stream_blocks;
+    const Kv4AttnArgs& a = tile ? ta : sa;
+    if (!tile) {
+        int total = 0;
+        for (int b0 = 0; b0 < a.requests; b0 += kJoinThreads) {
+            const int b = b0 + tid;
+            const int n = b < a.requests ? stream_list(stream_steps<D>(a, kv4_request(a, b))) * a.kv_heads : 0;
+            int before;
+            const int all = block_scan<kJoinWarps>(n, red, before);
+            if (b < a.requests) starts[b] = total + before;
+            total += all;
+        }
+        if (tid == 0) starts[a.requests] = total;
+        __syncthreads();
+        const RunCut run(total, stream_most(total, stream_grid));
+        const int items = total ? (run.ctas - 1) * a.max_cols : 0;
+        // few units: many shares each, which four warps take in turn
+        const int parts = a.requests * a.kv_heads * 4 <= run.ctas ? 4 : 1;
+        __shared__ float sums[kJoinWarps * D];
+        bool waited = false;
+        for (int i = blockIdx.x + stream_blocks * (warp / parts); i < items; i += stream_blocks * (kJoinWarps / parts)) {
+            const int cut = i / a.max_cols + 1, c = i % a.max_cols, at = run.start(cut);
+            int lo = 0, hi = a.requests - 1;  // the last request that starts at or before `at`
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (starts[mid] <= at) lo = mid;
+                else hi = mid - 1;
+            }
+            const Kv4Request r = kv4_request(a, lo);
+            if (c >= r.qn * a.group) continue;
+            const int n = stream_list(stream_steps<D>(a, r)), h = (at - starts[lo]) / n, u0 = starts[lo] + h * n;
+            const int first = run.owner(u0 + kStPad);  // of the unit's steps
+            if (at <= u0 + kStPad || first != cut - 1) continue;
+            // a CTA's slots: its first segment, its last; the unit is the first CTA's last, unless its run began in it
+            const float* s1 = a.part + (size_t)(2 * first) * ((size_t)kStRows * (D + 2));
+            const float* s0 = s1 + (run.start(first) < u0 ? (size_t)kStRows * (D + 2) : 0);
+            const int shares = run.owner(u0 + n - 1) - first + 1;
+            if (!waited) pdl_wait();
+            waited = true;
+            join_column<D>(a, r, h, c, s0, s1, shares, warp % parts, parts, sums + warp / parts * parts * D, 1 + warp / parts);
+        }
+        if (!waited) pdl_wait();  // a warp with nothing to join waits too: this grid's end stands for the whole call's
+        return;
+    }
+
     __shared__ float top_sm[kJoinRows], inv_sm[kJoinRows];
     __shared__ float wt[kJoinRows * kJoinShares];
     __shared__ float4 part_sm[kJoinThreads];
-    constexpr int TG = kv4_tile_rows(D) / kJoinRows;  // CTAs a tile cut
-    const bool tile = (int)blockIdx.x >= stream_grid - 1;
-    const Kv4AttnArgs& a = tile ? ta : sa;
-    const int cut = tile ? ((int)blockIdx.x - (stream_grid - 1)) / TG + 1 : (int)blockIdx.x + 1;
-    const int row0 = tile ? ((int)blockIdx.x - (stream_grid - 1)) % TG * kJoinRows : 0;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-
-    auto steps = [&](int b) { return stream_steps<D>(a, kv4_request(a, b)) * a.kv_heads; };
+    constexpr int TG = kv4_tile_rows(D) / kJoinRows;  // CTAs a cut
+    const int cut = ((int)blockIdx.x - stream_blocks) / TG + 1, row0 = ((int)blockIdx.x - stream_blocks) % TG * kJoinRows;
     int n0;
-    const int total = tile ? tile_list_total<D, kJoinWarps>(a, red, few, n0, [](int, const Kv4Request&, const TileUnit&, int) {})
-                           : list_total<kJoinWarps>(a.requests, red, n0, steps);
-    const RunCut run(total, tile ? tile_grid : stream_most(total, stream_grid));
-    // A CTA with nothing to join waits too: this grid's end stands for the whole call's.
+    const int total = tile_list_total<D, kJoinWarps>(a, red, few, n0, [](int, const Kv4Request&, const TileUnit&, int) {});
+    const RunCut run(total, tile_grid);
     if (total == 0 || cut >= run.ctas) {
         pdl_wait();
         return;
     }
     const int at = run.start(cut);
-    if (tile) tile_list_find<D, kJoinWarps>(a, red, pick, n0, at);
-    else list_find<kJoinWarps>(a.requests, red, pick, n0, at, steps);
+    tile_list_find<D, kJoinWarps>(a, red, pick, n0, at);
     const Kv4Request r = kv4_request(a, pick[0]);
-    int h, u0, n, e0 = 0, rows;
-    if (!tile) {
-        n = stream_steps<D>(a, r);
-        h = (at - pick[1]) / n;
-        u0 = pick[1] + h * n;
-        rows = r.qn * a.group;
-    } else {
-        const TileUnit t = tile_unit<D>(a, r, pick[2]);
-        u0 = pick[3], h = pick[4];
-        n = t.n, e0 = t.e0, rows = t.rows;
-    }
+    const TileUnit t = tile_unit<D>(a, r, pick[2]);
+    const int u0 = pick[3], h = pick[4], n = t.n, e0 = t.e0;
+    int rows = t.rows;
     const int first = run.owner(u0);
     if (u0 == at || first != cut - 1 || row0 >= rows) {
         pdl_wait();
@@ -63,7 +177,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
     }
     const int shares = run.owner(u0 + n - 1) - first + 1;
     rows = min(rows - row0, kJoinRows);
-    const int slot_rows = tile ? kv4_tile_rows(D) : kStRows;
+    constexpr int slot_rows = kv4_tile_rows(D);
     const size_t stride = (size_t)slot_rows * (D + 2);
     // a CTA's slots: its first segment, its last; the unit is the first CTA's last, unless it fills the run
     const float* s0 = a.part + (size_t)(2 * first + (run.start(first) != u0 ? 1 : 0)) * stride;
@@ -142,17 +256,21 @@ namespace {
 
 template <int D>
 cudaError_t join_launch(const Kv4AttnArgs& s, const Kv4AttnArgs* t, cudaStream_t stream) {
-    const int sg = kv4_stream_grid(D, s.max_cols), tg = t ? sm_count() : 1;
+    const int sg = kv4_stream_grid(D, s.max_cols), tg = t ? sm_count() : 1, blocks = sm_count();
+    const int smem = (s.requests + 1) * (int)sizeof(int);
+    cudaError_t e = func_attrs(reinterpret_cast<const void*>(kv4_join_kernel<D>), smem, false);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sg - 1 + (tg - 1) * (kv4_tile_rows(D) / kJoinRows), 1, 1);
+    cfg.gridDim = dim3(blocks + (tg - 1) * (kv4_tile_rows(D) / kJoinRows), 1, 1);
     cfg.blockDim = dim3(kJoinThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, s, t ? *t : s, sg, tg);
+    return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, s, t ? *t : s, sg, tg, blocks);
 }
 
 }  // namespace

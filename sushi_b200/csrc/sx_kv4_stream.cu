@@ -47,8 +47,8 @@ struct StreamLayout {
     static constexpr int TOTAL = BAR + kStWarps * kStStages * 8;
 };
 
-// A walk over the units' steps: request b, key head h; the unit's n steps begin at step `beg` of this
-// CTA's run (negative where the unit began in an earlier CTA's).
+// A walk over the units' steps: request b, key head h; the unit's n steps (n = 0, or the empty ones among
+// them) begin at step `beg` of this CTA's run (negative where the unit began in an earlier CTA's).
 struct StreamCursor {
     Kv4Request r;
     int b, h, n, beg;
@@ -63,7 +63,7 @@ __device__ __forceinline__ void stream_seek(const Kv4AttnArgs& a, StreamCursor& 
             c.h = 0;
             c.b++;
             c.r = kv4_request(a, c.b);
-            c.n = stream_steps<D>(a, c.r);
+            c.n = stream_list(stream_steps<D>(a, c.r));
         }
     }
 }
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
             uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)r.q0 * a.heads * D);
             for (size_t i = 0; i < (size_t)r.qn * a.heads * D / 8; i++) o[i] = make_uint4(0, 0, 0, 0);
         }
-        return n * a.kv_heads;
+        return stream_list(n) * a.kv_heads;
     };
     int n0;
     const int total = list_total<kStWarps>(a.requests, red, n0, steps);
@@ -143,33 +143,76 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
     StreamCursor cur;
     cur.b = pick[0];
     cur.r = kv4_request(a, cur.b);
-    cur.n = stream_steps<D>(a, cur.r);
+    cur.n = stream_list(stream_steps<D>(a, cur.r));
     const int into = start - pick[1];
     cur.h = into / cur.n;
     cur.beg = cur.h * cur.n - into;
     StreamCursor ahead = cur;
 
-    // ---------------- this warp's ring: step warp + 4 k of the run in stage k % S
+    // ---------------- this warp's ring: step warp + 4 k of the run in stage k % S.  A step's page ids (a
+    // load of their own, lane by lane) and places are looked up a step ahead of its copies.
     uint32_t valid = 0;  // 4 bits a stage: the granules that were copied
-    int next = warp;
+    int next = warp, page = -1;
+    size_t place = 0;
+    auto look = [&]() {
+        page = -1;
+        while (next < len) {  // past the empty steps
+            stream_seek<D>(a, ahead, next);
+            const int skip = ahead.beg + kStPad - next;
+            if (skip <= 0) break;
+            next += (skip + kStWarps - 1) / kStWarps * kStWarps;
+        }
+        if (next < len) {
+            const int pos = ahead.r.lo + ((next - ahead.beg - kStPad) * GS + lane) * kKvGranule;
+            if (lane < GS && pos < ahead.r.hi) page = a.table[ahead.b * a.tstride + (pos >> a.shift)];
+            place = kv4_granule<D>(0, a.kv_heads, ahead.h, a.page_size, pos & (a.page_size - 1));
+        }
+    };
+    const size_t page_bytes = kv4_granule<D>(1, a.kv_heads, 0, a.page_size, 0);
     auto issue = [&](int st) {
         if (next < len) {
-            stream_seek<D>(a, ahead, next);
-            const int pos = ahead.r.lo + ((next - ahead.beg) * GS + (lane < GS ? lane : 0)) * kKvGranule;
-            int page = -1;
-            if (lane < GS && pos < ahead.r.hi) page = a.table[ahead.b * a.tstride + (pos >> a.shift)];
             const bool ok = page >= 0 && page < a.pages;
             const uint32_t m = __ballot_sync(0xffffffffu, ok);
             if (lane == 0) mbar_arrive_expect_tx(&bar[st], __popc(m) * L::GB);
             __syncwarp();
-            if (ok)
-                bulk_g2s(ring + st * L::STEP + lane * L::GB,
-                         a.pool + kv4_granule<D>(page, a.kv_heads, ahead.h, a.page_size, pos & (a.page_size - 1)), L::GB,
-                         &bar[st]);
+            if (ok) bulk_g2s(ring + st * L::STEP + lane * L::GB, a.pool + page * page_bytes + place, L::GB, &bar[st]);
             valid = (valid & ~(15u << (4 * st))) | (m << (4 * st));
+            next += kStWarps;
+            look();
         }
-        next += kStWarps;
     };
+    // a unit's query entries of this warp's columns, loaded while the unit before is merged (where the
+    // registers allow)
+    constexpr int E = D / 32, CW = COLS / kStWarps;  // entries a lane, columns a warp
+    constexpr bool EARLY = E * CW <= 8;
+    float x[CW][E];
+    auto load_columns = [&]() {
+        const int n = cur.r.qn * a.group;
+#pragma unroll
+        for (int w = 0; w < CW; w++) {
+            const int c = warp + w * kStWarps;
+#pragma unroll
+            for (int e = 0; e < E; e++) x[w][e] = 0.0f;
+            if (c < n) {
+                const int qi = c / a.group, hh = cur.h * a.group + c - qi * a.group;
+                const long long at = (cur.r.q0 + qi) * a.qts + hh * a.qhs + lane * E;
+                if (a.qvec && E >= 4) {
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        float v4[4];
+                        load_act4(a.q, (size_t)(at + e), a.dt, v4);
+#pragma unroll
+                        for (int j = 0; j < 4 && e + j < E; j++) x[w][e + j] = v4[j];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[w][e] = load_act(a.q, (size_t)(at + e), a.dt);
+                }
+            }
+        }
+    };
+    if (EARLY) load_columns();
+    look();
 #pragma unroll
     for (int i = 0; i < kStStages; i++) issue(i);
 
@@ -187,37 +230,16 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
     uint32_t parity = 0;
     bool alive = true;
     for (int pos = 0; pos < len;) {
-        stream_seek<D>(a, cur, pos);
         const int seg_end = min(len, cur.beg + cur.n);
         const Kv4Request r = cur.r;
-        const int ncols = r.qn * a.group;
+        const int ncols = r.qn * a.group, beg = cur.beg + kStPad, n = cur.n - kStPad, head = cur.h;
+        const int from = max(pos, beg);  // steps [from, seg_end) are this CTA's
+        if (from >= seg_end) break;      // the run ends among the unit's empty steps
+        if (mine < from) mine += (from - mine + kStWarps - 1) / kStWarps * kStWarps;
 
         // ---------------- the unit's query columns: power-of-two scale, F16, fragment order
+        if (!EARLY) load_columns();
         __syncthreads();
-        constexpr int E = D / 32, CW = COLS / kStWarps;  // entries a lane, columns a warp
-        float x[CW][E];
-#pragma unroll
-        for (int w = 0; w < CW; w++) {
-            const int c = warp + w * kStWarps;
-#pragma unroll
-            for (int e = 0; e < E; e++) x[w][e] = 0.0f;
-            if (c < ncols) {
-                const int qi = c / a.group, hh = cur.h * a.group + c - qi * a.group;
-                const long long at = (r.q0 + qi) * a.qts + hh * a.qhs + lane * E;
-                if (a.qvec && E >= 4) {
-#pragma unroll
-                    for (int e = 0; e < E; e += 4) {
-                        float v4[4];
-                        load_act4(a.q, (size_t)(at + e), a.dt, v4);
-#pragma unroll
-                        for (int j = 0; j < 4 && e + j < E; j++) x[w][e + j] = v4[j];
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < E; e++) x[w][e] = load_act(a.q, (size_t)(at + e), a.dt);
-                }
-            }
-        }
 #pragma unroll
         for (int w = 0; w < CW; w++) {
             const int c = warp + w * kStWarps;
@@ -470,13 +492,18 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
         };
         for (; mine < seg_end; mine += kStWarps) {
             if (alive) alive = mbar_wait(&bar[stage], parity, DEV_TIMEOUT_FULL);
-            const int p0 = r.lo + (mine - cur.beg) * GS * kKvGranule;
+            const int p0 = r.lo + (mine - beg) * GS * kKvGranule;
             const uint32_t vm = (valid >> (4 * stage)) & 15u;
             if (p0 >= full_lo && p0 <= full_hi && vm == (1u << GS) - 1) step(ring + stage * L::STEP, p0, vm, std::true_type());
             else step(ring + stage * L::STEP, p0, vm, std::false_type());
             __syncwarp();
             issue(stage);
             if (++stage == kStStages) stage = 0, parity ^= 1u;
+        }
+
+        if (seg_end < len) {
+            stream_seek<D>(a, cur, seg_end);
+            if (EARLY) load_columns();
         }
 
         // ---------------- the warps' sums into one: common reference, then f32 adds in warp order
@@ -496,7 +523,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                 }
             }
         __syncthreads();
-        const bool whole = pos == cur.beg && seg_end == cur.beg + cur.n;
+        const bool whole = from == beg && seg_end == beg + n;
         float* slot = a.part + (size_t)(2 * cta + (pos == 0 ? 0 : 1)) * (kStRows * (D + 2));
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -538,7 +565,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                 }
                 if (whole) {
                     const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-                    const size_t at = ((size_t)(r.q0 + c / a.group) * a.heads + cur.h * a.group + c % a.group) * D + ch;
+                    const size_t at = ((size_t)(r.q0 + c / a.group) * a.heads + head * a.group + c % a.group) * D + ch;
                     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at) =
                         make_uint4(pack_act2(v[0] * inv, v[1] * inv, a.dt), pack_act2(v[2] * inv, v[3] * inv, a.dt),
                                    pack_act2(v[4] * inv, v[5] * inv, a.dt), pack_act2(v[6] * inv, v[7] * inv, a.dt));

@@ -67,8 +67,10 @@ def test_cache_refusals(L, kw, want):
         (dict(heads=0), "SX_ERR_BAD_SHAPE"),
         (dict(heads=7), "SX_ERR_BAD_SHAPE"),
         (dict(requests=0), "SX_ERR_BAD_SHAPE"),
+        (dict(requests=16385), "SX_ERR_BAD_SHAPE"),
         (dict(width=0), "SX_ERR_BAD_SHAPE"),
         (dict(stride=3), "SX_ERR_BAD_SHAPE"),
+        (dict(requests=1 << 14, width=1 << 20, stride=1 << 20), "SX_ERR_BAD_SHAPE"),
         (dict(requests=1 << 20, width=1 << 10, stride=1 << 10), "SX_ERR_BAD_SHAPE"),
         (dict(max_q=0), "SX_ERR_BAD_SHAPE"),
         (dict(window=-1), "SX_ERR_BAD_SHAPE"),
