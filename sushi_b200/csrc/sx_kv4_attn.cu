@@ -1,6 +1,6 @@
 // sx_kv4_attention: admission, and the choice between its two kernels, request by request on the
-// device: at most max_cols (row, query head) pairs a key head go to the streaming kernel, whose MMAs
-// carry 8 or 16 columns, the rest to the tile kernel, whose carry 128 rows.
+// device: at most kStMostPairs (row, query head) pairs a key head go to the streaming kernel, whose units
+// carry 8 or 16 of them, the rest to the tile kernel, whose carry 256.
 #include <cuda_runtime.h>
 #include <climits>
 #include <cmath>
@@ -11,11 +11,15 @@ using namespace sx;
 
 namespace {
 
-// The widest request of a call, and the pairs up to which its requests are the streaming kernel's.
+constexpr int kStMostPairs = 64;
+
+// The widest request of a call, in pairs a key head.
 long long most_pairs(const sx_kv4* c, int heads, int max_q) { return (long long)max_q * (heads / c->kv_heads); }
+// The columns of a streaming unit: 16 where a single row has more than 8 pairs or where every request is
+// the streaming kernel's and some have more than 8; 8 otherwise (a column tile less to multiply by).
 int stream_cols(const sx_kv4* c, int heads, int max_q) {
     const long long most = most_pairs(c, heads, max_q);
-    return heads / c->kv_heads > 8 || (most > 8 && most <= 16) ? 16 : 8;
+    return heads / c->kv_heads > 8 || (most > 8 && most <= kStMostPairs) ? 16 : 8;
 }
 
 // The workspace: the two partial slots of every CTA, the streaming kernel's (16 columns), then the
@@ -32,7 +36,7 @@ size_t sx_kv4_attention_workspace_bytes(const sx_kv4* cache, int32_t requests, i
     (void)requests, (void)tokens;
     if (!cache || !kv4_dim_ok(cache->head_dim) || cache->kv_heads < 1 || heads < cache->kv_heads || max_q < 1) return 0;
     const int D = cache->head_dim, cols = stream_cols(cache, heads, max_q);
-    return stream_bytes(D, cols) + (most_pairs(cache, heads, max_q) > cols ? tile_bytes(D) : 0);
+    return stream_bytes(D, cols) + (most_pairs(cache, heads, max_q) > kStMostPairs ? tile_bytes(D) : 0);
 }
 
 sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q, int64_t q_token_stride,
@@ -47,11 +51,11 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
         table_stride < table_width || max_q < 1 || window < 0 || !std::isfinite(scale))
         return SX_ERR_BAD_SHAPE;
     // the work lists count steps (of 16 tokens at the smallest; tiles of keys) in 32 bits
-    if ((long long)requests * cache->kv_heads * ((long long)table_width * (cache->page_size / kKvGranule)) > INT_MAX)
+    if ((long long)requests * cache->kv_heads * (kStMostPairs / 8) * ((long long)table_width * (cache->page_size / kKvGranule)) > INT_MAX)
         return SX_ERR_BAD_SHAPE;
     const long long blocks = (long long)tokens * (heads / cache->kv_heads) / kv4_tile_rows(cache->head_dim) + requests;
     const long long tiles = (long long)table_width * cache->page_size / kv4_tile_keys(cache->head_dim) + 1;
-    if (most_pairs(cache, heads, max_q) > stream_cols(cache, heads, max_q) &&
+    if (most_pairs(cache, heads, max_q) > kStMostPairs &&
         (double)blocks * (double)tiles * cache->kv_heads > INT_MAX)
         return SX_ERR_BAD_SHAPE;
     if (tokens == 0) return SX_OK;
@@ -70,16 +74,17 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     a.group = heads / cache->kv_heads;
     a.qvec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     a.scale_log2 = (float)(scale * 1.4426950408889634), a.window = window;
-    a.max_cols = stream_cols(cache, heads, max_q);
+    a.max_cols = kStMostPairs;
+    a.cols = stream_cols(cache, heads, max_q);
     a.part = static_cast<float*>(workspace);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int D = cache->head_dim;
     cudaError_t e = kv4_stream_launch(a, D, s);
     if (e != cudaSuccess) return cuda_status(e, "kv4_attention stream launch");
-    if (most_pairs(cache, heads, max_q) <= a.max_cols)
+    if (most_pairs(cache, heads, max_q) <= kStMostPairs)
         return cuda_status(kv4_join_launch(a, nullptr, D, s), "kv4_attention join launch");
     Kv4AttnArgs t = a;
-    t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_bytes(D, a.max_cols));
+    t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_bytes(D, a.cols));
     e = kv4_tile_launch(t, D, s);
     if (e != cudaSuccess) return cuda_status(e, "kv4_attention tile launch");
     return cuda_status(kv4_join_launch(a, &t, D, s), "kv4_attention join launch");

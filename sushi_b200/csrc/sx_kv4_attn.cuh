@@ -22,6 +22,7 @@ struct Kv4AttnArgs {
     float scale_log2;  // scale * log2(e)
     int window;
     int max_cols;      // requests of at most this many (row, head) pairs a key head are the streaming kernel's
+    int cols;          // the pairs its units take: 8 or 16
     float* part;       // the kernel's partial slots, two a CTA (units that several CTAs share)
 };
 
@@ -76,7 +77,8 @@ struct RunCut {
     }
 };
 
-// Streaming kernel: a step is 256/D granules of one unit = (request, key head).  A unit that has steps
+// Streaming kernel: a step is 256/D granules of one unit = (request, key head, block of `cols` pairs; the
+// blocks of a key head follow one another, so all but the first find its cache in L2).  A unit that has steps
 // begins with kStPad empty ones, which stand for the time a CTA needs to begin and merge it (3 to 4 us, a
 // step of its four warps 0.4 us): without them the CTAs of short requests finished last (64 requests of
 // 1024 to 16384 keys: from 83 to 110 us).
@@ -88,6 +90,9 @@ __device__ __forceinline__ int stream_steps(const Kv4AttnArgs& a, const Kv4Reque
     constexpr int T = kKvGranule * (256 / D);
     if (r.qn * (long long)a.group > a.max_cols) return 0;
     return (r.hi - r.lo + T - 1) / T;
+}
+__device__ __forceinline__ int stream_blocks(const Kv4AttnArgs& a, const Kv4Request& r) {
+    return (r.qn * a.group + a.cols - 1) / a.cols;
 }
 __device__ __forceinline__ int stream_list(int steps) { return steps > 0 ? steps + kStPad : 0; }  // a unit's share of the list
 // Every warp of a CTA that runs has a step to take.
@@ -238,7 +243,7 @@ __device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.lau
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // The streaming kernel (sx_kv4_stream.cu); its grid.
-int kv4_stream_grid(int D, int max_cols);
+int kv4_stream_grid(int D, int cols);
 cudaError_t kv4_stream_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream);
 // The tile kernel (sx_kv4_tile.cu): one CTA an SM.
 cudaError_t kv4_tile_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream);

@@ -22,7 +22,7 @@ constexpr int kJoinShares = 64;  // shares whose weights are held at a time
 // One column of a unit the streaming kernel's CTAs shared, by one warp, or by `parts` warps of a group that
 // take the shares in turn and add up in `sums` (parts > 1; the group's barrier id).
 template <int D>
-__device__ __forceinline__ void join_column(const Kv4AttnArgs& a, const Kv4Request& r, int h, int c, const float* s0,
+__device__ __forceinline__ void join_column(const Kv4AttnArgs& a, const Kv4Request& r, int h, int pair, int c, const float* s0,
                                             const float* s1, int shares, int part, int parts, float* sums, int barrier) {
     constexpr int E = D / 32;  // channels a lane
     constexpr size_t STRIDE = (size_t)kStRows * (D + 2);
@@ -96,24 +96,29 @@ __device__ __forceinline__ void join_column(const Kv4AttnArgs& a, const Kv4Reque
     }
     const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
     uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) +
-                                              ((size_t)(r.q0 + c / a.group) * a.heads + h * a.group + c % a.group) * D + lane * E);
+                                              ((size_t)(r.q0 + pair / a.group) * a.heads + h * a.group + pair % a.group) * D + lane * E);
 #pragma unroll
     for (int e = 0; e < E; e += 2) o[e / 2] = pack_act2(v[e] * inv, v[e + 1] * inv, a.dt);
 }
 
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, Kv4AttnArgs ta, int stream_grid, int tile_grid,
-                                                                int stream_blocks) {
+                                                                int column_ctas) {
     extern __shared__ int starts[];  // [requests + 1] the first step of each request in the streaming kernel's list
     __shared__ int red[kJoinWarps], pick[5], few[kTlFew];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const bool tile = (int)blockIdx.x >= stream_blocks;
+    const bool tile = (int)blockIdx.x >= column_ctas;
     const Kv4AttnArgs& a = tile ? ta : sa;
     if (!tile) {
         int total = 0;
         for (int b0 = 0; b0 < a.requests; b0 += kJoinThreads) {
             const int b = b0 + tid;
-            const int n = b < a.requests ? stream_list(stream_steps<D>(a, kv4_request(a, b))) * a.kv_heads : 0;
+            int n = 0;
+            if (b < a.requests) {
+                const Kv4Request r = kv4_request(a, b);
+                n = stream_list(stream_steps<D>(a, r));
+                if (n > 0) n *= a.kv_heads * stream_blocks(a, r);
+            }
             int before;
             const int all = block_scan<kJoinWarps>(n, red, before);
             if (b < a.requests) starts[b] = total + before;
@@ -122,13 +127,13 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
         if (tid == 0) starts[a.requests] = total;
         __syncthreads();
         const RunCut run(total, stream_most(total, stream_grid));
-        const int items = total ? (run.ctas - 1) * a.max_cols : 0;
+        const int items = total ? (run.ctas - 1) * a.cols : 0;
         // few units: many shares each, which four warps take in turn
         const int parts = a.requests * a.kv_heads * 4 <= run.ctas ? 4 : 1;
         __shared__ float sums[kJoinWarps * D];
         bool waited = false;
-        for (int i = blockIdx.x + stream_blocks * (warp / parts); i < items; i += stream_blocks * (kJoinWarps / parts)) {
-            const int cut = i / a.max_cols + 1, c = i % a.max_cols, at = run.start(cut);
+        for (int i = blockIdx.x + column_ctas * (warp / parts); i < items; i += column_ctas * (kJoinWarps / parts)) {
+            const int cut = i / a.cols + 1, c = i % a.cols, at = run.start(cut);
             int lo = 0, hi = a.requests - 1;  // the last request that starts at or before `at`
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -136,8 +141,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
                 else hi = mid - 1;
             }
             const Kv4Request r = kv4_request(a, lo);
-            if (c >= r.qn * a.group) continue;
-            const int n = stream_list(stream_steps<D>(a, r)), h = (at - starts[lo]) / n, u0 = starts[lo] + h * n;
+            const int n = stream_list(stream_steps<D>(a, r)), u = (at - starts[lo]) / n, u0 = starts[lo] + u * n;
+            const int blocks = stream_blocks(a, r), h = u / blocks, pair = (u - h * blocks) * a.cols + c;
+            if (pair >= r.qn * a.group) continue;
             const int first = run.owner(u0 + kStPad);  // of the unit's steps
             if (at <= u0 + kStPad || first != cut - 1) continue;
             // a CTA's slots: its first segment, its last; the unit is the first CTA's last, unless its run began in it
@@ -146,7 +152,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
             const int shares = run.owner(u0 + n - 1) - first + 1;
             if (!waited) pdl_wait();
             waited = true;
-            join_column<D>(a, r, h, c, s0, s1, shares, warp % parts, parts, sums + warp / parts * parts * D, 1 + warp / parts);
+            join_column<D>(a, r, h, pair, c, s0, s1, shares, warp % parts, parts, sums + warp / parts * parts * D, 1 + warp / parts);
         }
         if (!waited) pdl_wait();  // a warp with nothing to join waits too: this grid's end stands for the whole call's
         return;
@@ -156,7 +162,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(Kv4AttnArgs sa, 
     __shared__ float wt[kJoinRows * kJoinShares];
     __shared__ float4 part_sm[kJoinThreads];
     constexpr int TG = kv4_tile_rows(D) / kJoinRows;  // CTAs a cut
-    const int cut = ((int)blockIdx.x - stream_blocks) / TG + 1, row0 = ((int)blockIdx.x - stream_blocks) % TG * kJoinRows;
+    const int cut = ((int)blockIdx.x - column_ctas) / TG + 1, row0 = ((int)blockIdx.x - column_ctas) % TG * kJoinRows;
     int n0;
     const int total = tile_list_total<D, kJoinWarps>(a, red, few, n0, [](int, const Kv4Request&, const TileUnit&, int) {});
     const RunCut run(total, tile_grid);
@@ -256,7 +262,7 @@ namespace {
 
 template <int D>
 cudaError_t join_launch(const Kv4AttnArgs& s, const Kv4AttnArgs* t, cudaStream_t stream) {
-    const int sg = kv4_stream_grid(D, s.max_cols), tg = t ? sm_count() : 1, blocks = sm_count();
+    const int sg = kv4_stream_grid(D, s.cols), tg = t ? sm_count() : 1, blocks = sm_count();
     const int smem = (s.requests + 1) * (int)sizeof(int);
     cudaError_t e = func_attrs(reinterpret_cast<const void*>(kv4_join_kernel<D>), smem, false);
     if (e != cudaSuccess) return e;

@@ -1,7 +1,7 @@
 // Attention over the 4-bit cache for requests of few rows: one token, a few drafted ones.
 //
-// A unit is one request and key head; its columns are the (row, query head) pairs that read that key
-// head, at most 8 NT.  With 16 keys on the M axis and the columns on the N axis of m16n8k16:
+// A unit is one request and key head; its columns are (row, query head) pairs that read that key head, 8 NT
+// at most (more pairs make more units).  With 16 keys on the M axis and the columns on the N axis of m16n8k16:
 //   S^T[key][col] = sum over groups g of  s_kg * (codes . q) + m_kg * (sum of q in g)
 //   O^T[channel][col] = codes^T . (P * s_g) + sum over keys of P * m_g
 // so the products take the codes themselves: a code masked out of its word is the F16 subnormal
@@ -47,23 +47,32 @@ struct StreamLayout {
     static constexpr int TOTAL = BAR + kStWarps * kStStages * 8;
 };
 
-// A walk over the units' steps: request b, key head h; the unit's n steps (n = 0, or the empty ones among
+// A walk over the units' steps: request b, key head h, block k of its blocks; the unit's n steps (n = 0, or the empty ones among
 // them) begin at step `beg` of this CTA's run (negative where the unit began in an earlier CTA's).
 struct StreamCursor {
     Kv4Request r;
-    int b, h, n, beg;
+    int b, h, k, blocks, n, beg;
 };
+
+template <int D>
+__device__ __forceinline__ void stream_load(const Kv4AttnArgs& a, StreamCursor& c) {
+    c.r = kv4_request(a, c.b);
+    c.n = stream_list(stream_steps<D>(a, c.r));
+    c.blocks = stream_blocks(a, c.r);
+}
 
 // Moves the cursor forward to the unit that holds step i of the run.
 template <int D>
 __device__ __forceinline__ void stream_seek(const Kv4AttnArgs& a, StreamCursor& c, int i) {
     while (i >= c.beg + c.n) {
         c.beg += c.n;
-        if (++c.h >= a.kv_heads || c.n == 0) {
-            c.h = 0;
-            c.b++;
-            c.r = kv4_request(a, c.b);
-            c.n = stream_list(stream_steps<D>(a, c.r));
+        if (++c.k >= c.blocks || c.n == 0) {
+            c.k = 0;
+            if (++c.h >= a.kv_heads || c.n == 0) {
+                c.h = 0;
+                c.b++;
+                stream_load<D>(a, c);
+            }
         }
     }
 }
@@ -126,7 +135,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
             uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)r.q0 * a.heads * D);
             for (size_t i = 0; i < (size_t)r.qn * a.heads * D / 8; i++) o[i] = make_uint4(0, 0, 0, 0);
         }
-        return stream_list(n) * a.kv_heads;
+        return n > 0 ? stream_list(n) * a.kv_heads * stream_blocks(a, r) : 0;
     };
     int n0;
     const int total = list_total<kStWarps>(a.requests, red, n0, steps);
@@ -142,11 +151,12 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
     list_find<kStWarps>(a.requests, red, pick, n0, start, steps);
     StreamCursor cur;
     cur.b = pick[0];
-    cur.r = kv4_request(a, cur.b);
-    cur.n = stream_list(stream_steps<D>(a, cur.r));
+    stream_load<D>(a, cur);
     const int into = start - pick[1];
-    cur.h = into / cur.n;
-    cur.beg = cur.h * cur.n - into;
+    const int unit = into / cur.n;
+    cur.h = unit / cur.blocks;
+    cur.k = unit - cur.h * cur.blocks;
+    cur.beg = unit * cur.n - into;
     StreamCursor ahead = cur;
 
     // ---------------- this warp's ring: step warp + 4 k of the run in stage k % S.  A step's page ids (a
@@ -187,14 +197,14 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
     constexpr bool EARLY = E * CW <= 8;
     float x[CW][E];
     auto load_columns = [&]() {
-        const int n = cur.r.qn * a.group;
+        const int n = cur.r.qn * a.group, h = cur.h, e0 = cur.k * a.cols;
 #pragma unroll
         for (int w = 0; w < CW; w++) {
-            const int c = warp + w * kStWarps;
+            const int c = e0 + warp + w * kStWarps;
 #pragma unroll
             for (int e = 0; e < E; e++) x[w][e] = 0.0f;
-            if (c < n) {
-                const int qi = c / a.group, hh = cur.h * a.group + c - qi * a.group;
+            if (c < n && warp + w * kStWarps < a.cols) {
+                const int qi = c / a.group, hh = h * a.group + c - qi * a.group;
                 const long long at = (cur.r.q0 + qi) * a.qts + hh * a.qhs + lane * E;
                 if (a.qvec && E >= 4) {
 #pragma unroll
@@ -232,7 +242,9 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
     for (int pos = 0; pos < len;) {
         const int seg_end = min(len, cur.beg + cur.n);
         const Kv4Request r = cur.r;
-        const int ncols = r.qn * a.group, beg = cur.beg + kStPad, n = cur.n - kStPad, head = cur.h;
+        const int beg = cur.beg + kStPad, n = cur.n - kStPad, head = cur.h;
+        const int e0 = cur.k * a.cols;  // the unit's first pair
+        const int ncols = min(a.cols, r.qn * a.group - e0);
         const int from = max(pos, beg);  // steps [from, seg_end) are this CTA's
         if (from >= seg_end) break;      // the run ends among the unit's empty steps
         if (mine < from) mine += (from - mine + kStWarps - 1) / kStWarps * kStWarps;
@@ -277,7 +289,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
             for (int j = 0; j < 2; j++) {
                 const int c = nt * 8 + 2 * t + j;
                 chs[nt][j] = ch_sm[c];
-                qpos[nt][j] = r.pos0 + (c < ncols ? c / a.group : 0);
+                qpos[nt][j] = r.pos0 + (e0 + (c < ncols ? c : 0)) / a.group;
 #pragma unroll
                 for (int gr = 0; gr < G; gr++) qs[nt][j][gr] = qs_sm[c * G + gr];
             }
@@ -565,7 +577,8 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                 }
                 if (whole) {
                     const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-                    const size_t at = ((size_t)(r.q0 + c / a.group) * a.heads + head * a.group + c % a.group) * D + ch;
+                    const int pair = e0 + c;
+                    const size_t at = ((size_t)(r.q0 + pair / a.group) * a.heads + head * a.group + pair % a.group) * D + ch;
                     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at) =
                         make_uint4(pack_act2(v[0] * inv, v[1] * inv, a.dt), pack_act2(v[2] * inv, v[3] * inv, a.dt),
                                    pack_act2(v[4] * inv, v[5] * inv, a.dt), pack_act2(v[6] * inv, v[7] * inv, a.dt));
@@ -605,15 +618,15 @@ cudaError_t stream_launch(const Kv4AttnArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-int kv4_stream_grid(int D, int max_cols) {
-    const bool one = max_cols <= 8;
+int kv4_stream_grid(int D, int cols) {
+    const bool one = cols <= 8;
     if (D == 64) return one ? stream_ctas<64, 1>() : stream_ctas<64, 2>();
     if (D == 128) return one ? stream_ctas<128, 1>() : stream_ctas<128, 2>();
     return one ? stream_ctas<256, 1>() : stream_ctas<256, 2>();
 }
 
 cudaError_t kv4_stream_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream) {
-    const bool one = a.max_cols <= 8;
+    const bool one = a.cols <= 8;
     if (D == 64) return one ? stream_launch<64, 1>(a, stream) : stream_launch<64, 2>(a, stream);
     if (D == 128) return one ? stream_launch<128, 1>(a, stream) : stream_launch<128, 2>(a, stream);
     return one ? stream_launch<256, 1>(a, stream) : stream_launch<256, 2>(a, stream);
