@@ -468,3 +468,18 @@ def test_refusals_by_name():
         sx().kv4_write(st.cache, st.k, st.v, st.slots[:5])
     with pytest.raises(E, match="SX_ERR_BAD_DTYPE"):
         sx().kv4_read(st.cache, st.slots, torch.int32)
+
+
+def test_the_example_layer():
+    """Prompt, decode and graph steps of an EXL3 attention layer; a decoded row against the same row of a
+    whole prompt: bf16 activations through two projections and both attention kernels, each rounded
+    to 2^-8, four roundings deep."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "kv4_layer.py")
+    spec = importlib.util.spec_from_file_location("kv4_layer", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main() < 4 * 2.0 ** -8
+    assert sx().device_error() == 0
