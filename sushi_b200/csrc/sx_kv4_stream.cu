@@ -8,7 +8,9 @@
 // code * 2^-24 (or code * 2^-20 for every second nibble), exact, with no conversion.  The query is
 // scaled by a power of two per column (its largest entry to [2^13, 2^14)) and by 1/16 where the
 // nibble brings 16, and rounded to F16 (exact for bf16 and f16 entries within 2^24 of the largest).
-// P * s is rounded to F16 once; m, sums and accumulators are f32.
+// P * s is rounded to F16 once (bf16 calls: the output's own rounding is eight times as coarse), or kept
+// in two F16 parts with a second product (FINE, F16 calls: with one part the output's error was twice its
+// rounding's); m, sums and accumulators are f32.
 //
 // The softmax reference of a column is kept so that P * s <= 2^15, whatever the values' magnitude:
 // it moves (one vote a step) only when a score or a step would pass that, with 2^4 to spare.
@@ -109,7 +111,7 @@ __host__ __device__ constexpr int stream_resident() {
     return NT == 1 && D <= 128 ? 3 : 2;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool FINE>
 __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stream_kernel(Kv4AttnArgs a) {
     using L = StreamLayout<D, NT>;
     constexpr int G = L::G, GS = L::GS, COLS = L::COLS;
@@ -448,7 +450,8 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
 #pragma unroll
             for (int gi = 0; gi < GS; gi++) {
                 const uint8_t* gran = st + gi * L::GB;
-                uint32_t pb[G][NT][2];
+                uint32_t pb[G][NT][2];                  // P * s
+                [[maybe_unused]] uint32_t pl[G][NT][2];  // FINE: what its rounding left
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float p[4];
@@ -471,6 +474,11 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                             mn[gr][nt][1] = fmaf(b1, m1, mn[gr][nt][1]);
                             const __half2 h2 = __floats2half2_rn(a0, a1);
                             pb[gr][nt][rr] = movmatrix(*reinterpret_cast<const uint32_t*>(&h2));
+                            if constexpr (FINE) {
+                                const float2 r2 = __half22float2(h2);
+                                const __half2 l2 = __floats2half2_rn(a0 - r2.x, a1 - r2.y);
+                                pl[gr][nt][rr] = movmatrix(*reinterpret_cast<const uint32_t*>(&l2));
+                            }
                         }
                 }
                 uint32_t vw[4][G];
@@ -495,9 +503,13 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                     for (int mt = 0; mt < 4; mt++) {
                         const uint32_t xx = w01[mt >> 1] >> (8 * (mt & 1)), yy = w23[mt >> 1] >> (8 * (mt & 1));
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
+                        for (int nt = 0; nt < NT; nt++) {
                             mma16816(o[gr][mt][nt], xx & 0x000f000fu, xx & 0x00f000f0u, yy & 0x000f000fu, yy & 0x00f000f0u,
                                      pb[gr][nt][0], pb[gr][nt][1]);
+                            if constexpr (FINE)
+                                mma16816(o[gr][mt][nt], xx & 0x000f000fu, xx & 0x00f000f0u, yy & 0x000f000fu, yy & 0x00f000f0u,
+                                         pl[gr][nt][0], pl[gr][nt][1]);
+                        }
                     }
                 }
             }
@@ -609,7 +621,7 @@ int stream_ctas() {
 template <int D, int NT>
 cudaError_t stream_launch(const Kv4AttnArgs& a, cudaStream_t stream) {
     using L = StreamLayout<D, NT>;
-    auto kern = kv4_stream_kernel<D, NT>;
+    auto kern = a.dt == SX_DT_F16 ? kv4_stream_kernel<D, NT, true> : kv4_stream_kernel<D, NT, false>;
     cudaError_t e = func_attrs(reinterpret_cast<const void*>(kern), L::TOTAL, false);
     if (e != cudaSuccess) return e;
     kern<<<stream_ctas<D, NT>(), kStThreads, L::TOTAL, stream>>>(a);
