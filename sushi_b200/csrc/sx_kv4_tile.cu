@@ -364,31 +364,45 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             const int qpos = r.pos0 + qi;
 
             // the query row: scaled by a power of two (largest entry to [2^13, 2^14)), F16, chunk order
+            // (a thread without a pair reads the block's first and takes 0 of it; 16 loads in flight)
             const long long at = (r.q0 + qi) * a.qts + head * a.qhs;
-            auto load8q = [&](int c, float (&x)[8]) {
-                if (!live) {
+            const uint16_t* qrow = static_cast<const uint16_t*>(a.q) + at;
+            auto load_q = [&](int c0, uint4 (&w)[8]) {
+                if (a.qvec) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = 0.0f;
-                } else if (a.qvec) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at + c);
-                    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const uint16_t h = (uint16_t)(ww[i >> 1] >> (16 * (i & 1)));
-                        x[i] = a.dt == 1 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
-                    }
+                    for (int i = 0; i < 8; i++) w[i] = *reinterpret_cast<const uint4*>(qrow + c0 + i * 8);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = load_act(a.q, (size_t)(at + c + i), a.dt);
+                    for (int i = 0; i < 8; i++) {
+                        const uint16_t* p = qrow + c0 + i * 8;
+                        w[i] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16,
+                                          p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+                    }
                 }
             };
-            float top = 0.0f;
-#pragma unroll 8
-            for (int c = 0; c < D; c += 8) {
-                float x[8];
-                load8q(c, x);
+            auto widen = [&](const uint4& w, float (&x)[8]) {
+                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[i]));
+                for (int i = 0; i < 8; i++) {
+                    const uint16_t h = (uint16_t)(ww[i >> 1] >> (16 * (i & 1)));
+                    x[i] = a.dt == 1 ? __half2float(__ushort_as_half(h)) : __bfloat162float(__ushort_as_bfloat16(h));
+                }
+            };
+            constexpr bool HOLD = D <= 128;  // the whole row in registers between the two passes
+            uint4 qw[HOLD ? D / 64 : 1][8];
+            float top = 0.0f;
+#pragma unroll
+            for (int b = 0; HOLD && b < D / 64; b++) load_q(b * 64, qw[HOLD ? b : 0]);
+#pragma unroll
+            for (int b = 0; b < D / 64; b++) {
+                if (!HOLD) load_q(b * 64, qw[0]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float x[8];
+                    widen(qw[HOLD ? b : 0][i], x);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
+                }
             }
             int k2 = 0;
             if (top > 0.0f && top < 3.0e38f) k2 = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -120), 120);
@@ -396,18 +410,22 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             const float up = copysignf(__uint_as_float((uint32_t)(k2 + 127) << 23), a.scale_log2);
             // (a scale of 0 keeps c above 0: -inf c is then -inf, and what is left of the scores adds nothing)
             const float c = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k2) << 23), 1.0e-30f);
-#pragma unroll 8
-            for (int ch = 0; ch < D; ch += 8) {
-                float x[8];
-                load8q(ch, x);
-                uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const __half2 h = __floats2half2_rn(x[i] * up, x[i + 4] * up);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int b = 0; b < D / 64; b++) {
+                if (!HOLD) load_q(b * 64, qw[0]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    float x[8];
+                    widen(qw[HOLD ? b : 0][i], x);
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const __half2 h = __floats2half2_rn(x[k] * up, x[k + 4] * up);
+                        w[k] = live ? *reinterpret_cast<const uint32_t*>(&h) : 0u;
+                    }
+                    *reinterpret_cast<uint4*>(smem + L::Q + mt * L::Q_TILE + b * 16384 + sw128_offset(row, i * 8)) =
+                        make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                *reinterpret_cast<uint4*>(smem + L::Q + mt * L::Q_TILE + (ch >> 6) * 16384 + sw128_offset(row, ch & 63)) =
-                    make_uint4(w[0], w[1], w[2], w[3]);
             }
             fence_proxy_async_smem();
             __syncwarp();
