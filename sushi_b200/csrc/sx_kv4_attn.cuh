@@ -100,6 +100,10 @@ __device__ __forceinline__ int stream_most(int total, int grid) { return min(gri
 
 // Tile kernel: a step is a tile of kv4_tile_keys(D) keys of one unit = (request, key head, block of
 // kv4_tile_rows(D) (row, query head) pairs).
+// A unit that has tiles begins with kTlPad empty ones in the list, which stand for the time a CTA needs to
+// begin and end it (about 8 us, a tile 3.6): without them the CTAs of short units finished last (a mixed
+// step: 172 us where the others took 110 to 140).
+constexpr int kTlPad = 2;
 __host__ __device__ constexpr int kv4_tile_rows(int D) { return D == 256 ? 128 : 256; }
 __host__ __device__ constexpr int kv4_tile_keys(int D) { return D == 256 ? 64 : 128; }
 
@@ -119,6 +123,8 @@ __device__ __forceinline__ TileUnit tile_unit(const Kv4AttnArgs& a, const Kv4Req
     t.n = hi > t.lo ? (hi - t.lo + kv4_tile_keys(D) - 1) / kv4_tile_keys(D) : 0;
     return t;
 }
+
+__device__ __forceinline__ int tile_list(int tiles) { return tiles > 0 ? tiles + kTlPad : 0; }  // a unit's share of the list
 
 // A request's blocks; 0 for the streaming kernel's requests.
 template <int D>
@@ -194,7 +200,7 @@ __device__ __forceinline__ int tile_list_total(const Kv4AttnArgs& a, int* red, i
         for (int u = u0; u < blocks; u += du) {
             const TileUnit t = tile_unit<D>(a, r, u);
             each(b, r, t, u);
-            n += t.n;
+            n += tile_list(t.n);
         }
         return n;
     };
@@ -217,12 +223,12 @@ __device__ __forceinline__ void tile_list_find(const Kv4AttnArgs& a, int* red, i
         const Kv4Request r = kv4_request(a, b);
         const int blocks = tile_blocks<D>(a, r);
         int n = 0;
-        for (int u = 0; u < blocks; u++) n += tile_unit<D>(a, r, u).n;
+        for (int u = 0; u < blocks; u++) n += tile_list(tile_unit<D>(a, r, u).n);
         return n * a.kv_heads;
     });
     const Kv4Request r = kv4_request(a, pick[0]);
     const int blocks = tile_blocks<D>(a, r);
-    auto unit = [&](int u) { return u < blocks ? tile_unit<D>(a, r, u).n : 0; };
+    auto unit = [&](int u) { return u < blocks ? tile_list(tile_unit<D>(a, r, u).n) : 0; };
     int head = 0, before;
     for (int u0 = 0; u0 < blocks; u0 += W * 32) head += block_scan<W>(unit(u0 + threadIdx.x), red, before);
     const int h = (at - pick[1]) / head, first = pick[1] + h * head;

@@ -60,8 +60,8 @@ struct TileLayout {
     static_assert(ALLOC <= 227 * 1024, "fits a CTA");
 };
 
-// A walk over the units' tiles: the unit's first tile is step `beg` of this CTA's run (negative where it
-// began in an earlier CTA's).
+// A walk over the units' tiles: the unit's first tile is tile `beg` of this CTA's (negative where an earlier
+// CTA has it).
 struct TileCursor {
     Kv4Request r;
     TileUnit t;
@@ -77,7 +77,7 @@ __device__ __forceinline__ void tile_load(const Kv4AttnArgs& a, TileCursor& c) {
     if (c.blocks) c.t = tile_unit<D>(a, c.r, 0);
 }
 
-// Moves the cursor forward to the unit that holds tile i of the run.
+// Moves the cursor forward to the unit that holds this CTA's tile i.
 template <int D>
 __device__ __forceinline__ void tile_seek(const Kv4AttnArgs& a, TileCursor& c, int i) {
     while (i >= c.beg + c.t.n) {
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     constexpr int G = L::G, MT = L::MT, NK = L::NK, NG = L::NG;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_slot;
-    __shared__ int red[L::THREADS / 32], pick[5], few[kTlFew];
+    __shared__ int red[L::THREADS / 32], pick[5], few[kTlFew], run_tiles;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + L::BAR);  // [widening warps][RING]
@@ -322,8 +322,24 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
         return;
     }
     const int start = run.start(cta);
-    const int len = run.start(cta + 1) - start;  // this CTA's run
     tile_list_find<D, W>(a, red, pick, n0, start);
+    TileCursor cur;
+    cur.b = pick[0];
+    tile_load<D>(a, cur);
+    cur.u = pick[2], cur.h = pick[4];
+    cur.beg = min(0, pick[3] + kTlPad - start);
+    cur.t = tile_unit<D>(a, cur.r, cur.u);
+    if (tid == 0) {
+        // the run's tiles, less the units' empty ones
+        const int end = run.start(cta + 1);
+        TileCursor c = cur;
+        int n = 0;
+        for (int p = pick[3]; p < end; p += tile_list(c.t.n)) {
+            if (p > pick[3]) tile_seek<D>(a, c, c.beg + c.t.n);
+            n += max(0, min(end, p + tile_list(c.t.n)) - max(start, p + kTlPad));
+        }
+        run_tiles = n;
+    }
     if (warp == L::MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512)
                      : "memory");
@@ -333,12 +349,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    TileCursor cur;
-    cur.b = pick[0];
-    tile_load<D>(a, cur);
-    cur.u = pick[2], cur.h = pick[4];
-    cur.beg = pick[3] - start;
-    cur.t = tile_unit<D>(a, cur.r, cur.u);
+    const int len = run_tiles;  // this CTA's tiles
 
     if (warp < L::SM_WARPS) {
         // ---------------- softmax: one thread a (row, head) pair of row tile `mt`
@@ -605,7 +616,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             pos = seg_end;
         }
     } else if (warp < L::MMA_WARP) {
-        // ---------------- widening: task q of the run is granule q % NG of tile q / (2 NG), its keys, then its values
+        // ---------------- widening: task q of the CTA's is granule q % NG of tile q / (2 NG), its keys, then its values
         const int w = warp - L::SM_WARPS;
         uint8_t* ring = smem + L::RAW + w * L::RING * L::HB;
         uint64_t* bar = raw_full + w * L::RING;
@@ -742,7 +753,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             pos = seg_end;
         }
         // the last commit of all: nothing of this CTA's is in flight when it frees its tensor memory
-        if (ok) mbar_wait(&vempty[(tiles - 1) % L::VST], ((tiles - 1) / L::VST) & 1, DEV_TIMEOUT_EMPTY);
+        if (ok && tiles > 0) mbar_wait(&vempty[(tiles - 1) % L::VST], ((tiles - 1) / L::VST) & 1, DEV_TIMEOUT_EMPTY);
     }
     pdl_wait();  // the join that follows waits for this grid: the streaming kernel's end is part of it
     tc_fence_before();
