@@ -79,7 +79,8 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     a.requests = requests, a.width = table_width, a.tstride = table_stride;
     a.group = heads / cache->kv_heads;
     a.qvec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
-    a.scale_log2 = (float)(scale * 1.4426950408889634), a.window = window;
+    a.scale_log2 = (float)(scale * 1.4426950408889634);
+    a.window = window > (1 << 30) ? 0 : window;  // wider than any cache: none (and positions less it stay in 32 bits)
     a.max_cols = kStMostPairs;
     a.cols = stream_cols(cache, heads, max_q);
     a.part = static_cast<float*>(workspace);

@@ -226,6 +226,17 @@ LENS = {
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 4, 7])
+def test_attention_of_long_units(d, group):
+    """Units of many tiles a CTA, whole and shared, so that every ring goes round several times."""
+    st = Step(d + group, d, torch.bfloat16, 8 * group, 8, 64, [(4100, 700), (900, 900), (2500, 300)])
+    first = st.run()
+    st.check(first)
+    assert torch.equal(st.run(), first)
+    assert sx().device_error() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("lens", list(LENS))
 @pytest.mark.parametrize("heads,kv_heads,page,window", [(1, 1, 16, 0), (8, 2, 64, 0), (7, 1, 32, 50), (32, 2, 128, 0),
@@ -236,7 +247,7 @@ def test_attention(d, dtype, lens, heads, kv_heads, page, window):
     assert sx().device_error() == 0
 
 
-@pytest.mark.parametrize("window", [1, 2, 16, 64, 65])
+@pytest.mark.parametrize("window", [1, 2, 16, 64, 65, 1 << 20, (1 << 31) - 1])
 def test_attention_windows(window):
     st = Step(window, 128, torch.bfloat16, 8, 2, 16, [(1, 1), (64, 1), (65, 2), (200, 150), (513, 1), (129, 129)], window)
     st.check(st.run())
