@@ -2,6 +2,7 @@
 // device: at most kStMostPairs (row, query head) pairs a key head go to the streaming kernel, whose units
 // carry 8 or 16 of them, the rest to the tile kernel, whose carry 256.
 #include <cuda_runtime.h>
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -57,12 +58,13 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
         table_stride < table_width || max_q < 1 || window < 0 || !std::isfinite(scale))
         return SX_ERR_BAD_SHAPE;
     // the work lists count steps (of 16 tokens at the smallest; tiles of keys) in 32 bits
-    if ((long long)requests * cache->kv_heads * (kStMostPairs / 8) * ((long long)table_width * (cache->page_size / kKvGranule)) > INT_MAX)
-        return SX_ERR_BAD_SHAPE;
+    const long long most = most_pairs(cache, heads, max_q);
+    const int cols = stream_cols(cache, heads, max_q);
+    const long long units = (long long)requests * cache->kv_heads * ((std::min<long long>(most, kStMostPairs) + cols - 1) / cols);
+    if ((double)units * ((double)table_width * (cache->page_size / kKvGranule) + kStPad) > INT_MAX) return SX_ERR_BAD_SHAPE;
     const long long blocks = (long long)tokens * (heads / cache->kv_heads) / kv4_tile_rows(cache->head_dim) + requests;
-    const long long tiles = (long long)table_width * cache->page_size / kv4_tile_keys(cache->head_dim) + 1;
-    if (most_pairs(cache, heads, max_q) > kStMostPairs &&
-        (double)blocks * (double)tiles * cache->kv_heads > INT_MAX)
+    const long long tiles = (long long)table_width * cache->page_size / kv4_tile_keys(cache->head_dim) + 1 + kTlPad;
+    if (most > kStMostPairs && (double)blocks * (double)tiles * cache->kv_heads > INT_MAX)
         return SX_ERR_BAD_SHAPE;
     if (tokens == 0) return SX_OK;
     if (!q || !cu_q || !kv_lens || !table || !out || !workspace) return SX_ERR_NULL_POINTER;
@@ -82,13 +84,13 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     a.scale_log2 = (float)(scale * 1.4426950408889634);
     a.window = window > (1 << 30) ? 0 : window;  // wider than any cache: none (and positions less it stay in 32 bits)
     a.max_cols = kStMostPairs;
-    a.cols = stream_cols(cache, heads, max_q);
+    a.cols = cols;
     a.part = static_cast<float*>(workspace);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int D = cache->head_dim;
     cudaError_t e = kv4_stream_launch(a, D, s);
     if (e != cudaSuccess) return cuda_status(e, "kv4_attention stream launch");
-    if (most_pairs(cache, heads, max_q) <= kStMostPairs)
+    if (most <= kStMostPairs)
         return cuda_status(kv4_join_launch(a, nullptr, D, s), "kv4_attention join launch");
     Kv4AttnArgs t = a;
     t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_bytes(D, a.cols));

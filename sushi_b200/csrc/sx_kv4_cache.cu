@@ -14,7 +14,8 @@ namespace sx {
 // the new table entries, each item finding its request by a binary search of the sums.  Every CTA
 // makes the sums for itself (8 bytes a request from L2), so the step is one launch in which no CTA
 // waits for another; a token on a new page takes the page from the stack itself rather than from the
-// table entry another CTA writes.  Bound by launch and load latency.
+// table entry another CTA writes.  Bound by launch and load latency (8 requests 2.7 us; 1024 requests with
+// 13 thousand new tokens 6.7 us).
 constexpr int kTablesThreads = 256;
 constexpr int kTablesItems = 4;           // tokens a thread
 
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kTablesThreads) block_tables_kernel(
 // (16-bit types), each group's minimum and maximum over its eight lanes by shuffles, one 32-bit word of
 // codes each.  Both kernels are HBM bound, one pass over the data.  The grid's y walks the tokens, so an
 // item's head and piece come from 32-bit arithmetic (a 64-bit division an item took most of the time:
-// 8192 tokens of 8 heads of 128, written and read back, 76 us with it).
+// 8192 tokens of 8 heads of 128, written and read back, 76 us with it, 37 us now: 2.3 TB/s of what has to move).
 constexpr int kKvThreads = 256;
 constexpr int kKvMostHeads = 65536;  // a token's items, and a CTA's, stay in 32 bits
 

