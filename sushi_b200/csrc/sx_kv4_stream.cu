@@ -15,6 +15,13 @@
 // The softmax reference of a column is kept so that P * s <= 2^15, whatever the values' magnitude:
 // it moves (one vote a step) only when a score or a step would pass that, with 2^4 to spare.
 //
+// The MMA's f32 sums are cut, not rounded, at each of their additions.  Over a long cache the codes' part
+// (codes are 0 to 15) and the minima's are hundreds of times their sum, the output, and a cut of 2^-24 of the
+// one at each granule grows with the length: at 131072 keys a CTA outputs were 5% off.  So every MOVE steps the
+// minima's part moves into the codes' sums, which are then of the output's size; the error no longer depends on
+// the length (131072 keys a CTA, relative: bf16 1.7e-3, of which the output's own rounding is 1.6e-3; F16
+// 2.7e-4 of 2.1e-4, 3.3e-4 with MOVE = 8).  64 requests of 1024 to 16384 keys: 110 us without, 114 with it.
+//
 // Work: the units' steps (4.5 KB of one head: 256/D granules of 16 tokens) laid end to end and cut
 // into equal runs, one a CTA, so ragged lengths balance; a CTA's warps take its steps in turn, each
 // with its own ring of bulk copies.  A unit that several CTAs share is joined by sx_kv4_join.cu.
@@ -119,6 +126,7 @@ template <int D, int NT, bool FINE>
 __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stream_kernel(Kv4AttnArgs a) {
     using L = StreamLayout<D, NT>;
     constexpr int G = L::G, GS = L::GS, COLS = L::COLS;
+    constexpr int MOVE = FINE ? 4 : 8;  // steps; an F16 output shows an error an eighth of bf16's
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int red[kStWarps], pick[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -518,15 +526,36 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                 }
             }
         };
-        for (; mine < seg_end; mine += kStWarps) {
-            if (alive) alive = mbar_wait(&bar[stage], parity, DEV_TIMEOUT_FULL);
-            const int p0 = r.lo + (mine - beg) * GS * kKvGranule;
-            const uint32_t vm = (valid >> (4 * stage)) & 15u;
-            if (p0 >= full_lo && p0 <= full_hi && vm == (1u << GS) - 1) step(ring + stage * L::STEP, p0, vm, std::true_type());
-            else step(ring + stage * L::STEP, p0, vm, std::false_type());
-            __syncwarp();
-            issue(stage);
-            if (++stage == kStStages) stage = 0, parity ^= 1u;
+        while (mine < seg_end) {
+            const int stop = min(seg_end, mine + MOVE * kStWarps);
+            for (; mine < stop; mine += kStWarps) {
+                if (alive) alive = mbar_wait(&bar[stage], parity, DEV_TIMEOUT_FULL);
+                const int p0 = r.lo + (mine - beg) * GS * kKvGranule;
+                const uint32_t vm = (valid >> (4 * stage)) & 15u;
+                if (p0 >= full_lo && p0 <= full_hi && vm == (1u << GS) - 1) step(ring + stage * L::STEP, p0, vm, std::true_type());
+                else step(ring + stage * L::STEP, p0, vm, std::false_type());
+                __syncwarp();
+                issue(stage);
+                if (++stage == kStStages) stage = 0, parity ^= 1u;
+            }
+            if (mine >= seg_end) break;
+            // the minima's part into the sums of codes
+#pragma unroll
+            for (int gr = 0; gr < G; gr++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        float y = mn[gr][nt][j];
+                        mn[gr][nt][j] = 0.0f;
+#pragma unroll
+                        for (int m = 4; m < 32; m <<= 1) y += __shfl_xor_sync(0xffffffffu, y, m);
+#pragma unroll
+                        for (int mt = 0; mt < 4; mt++) {
+                            o[gr][mt][nt][j] = fmaf(y, 5.9604644775390625e-08f, o[gr][mt][nt][j]);          // 2^-24
+                            o[gr][mt][nt][j + 2] = fmaf(y, 9.5367431640625e-07f, o[gr][mt][nt][j + 2]);  // 2^-20
+                        }
+                    }
         }
 
         if (seg_end < len) {

@@ -1,0 +1,66 @@
+"""Attention over long caches, held to bars that a lost key or a drifting sum breaks (tests/kv4_bars.py)."""
+
+import pytest
+import torch
+
+import kv4_bars as bars
+import kv4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def sx():
+    import sushi_b200
+
+    return sushi_b200
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+class Shared:
+    """Many requests over the same pages (one cache of n keys, values without a mean), the same query
+    rows in each: more units than the GPU has CTAs, so a CTA sums whole units."""
+
+    def __init__(self, seed, n, requests, rows, heads, kv_heads, d, dtype, page=64):
+        f = dict(generator=gen(seed), device="cuda")
+        pages = -(-n // page)
+        self.cache = sx().Kv4Cache(pages, kv_heads, d, page)
+        self.k, self.v = (torch.randn((n, kv_heads, d), **f).to(dtype) for _ in range(2))
+        ids = torch.randperm(pages, **f)
+        pos = torch.arange(n, device="cuda")
+        sx().kv4_write(self.cache, self.k, self.v, ids[pos // page] * page + pos % page)
+        self.table = ids.int()[None].repeat(requests, 1)
+        self.q = torch.randn((rows, heads, d), **f).to(dtype)
+        self.n, self.requests, self.rows, self.heads, self.kv_heads, self.d = n, requests, rows, heads, kv_heads, d
+
+    def run(self):
+        cu = [self.rows * b for b in range(self.requests + 1)]
+        return sx().kv4_attention(self.q.repeat(self.requests, 1, 1), self.cache, self.table, i32([self.n] * self.requests),
+                                  i32(cu), self.rows).reshape(self.requests, self.rows, self.heads, self.d)
+
+    def want(self):
+        k, v = ref.held(self.k)[0], ref.held(self.v)[0]
+        seen = torch.arange(self.n, device="cuda") <= torch.arange(self.n - self.rows, self.n, device="cuda")[:, None]
+        out = []
+        for h in range(self.heads):
+            kh = h // (self.heads // self.kv_heads)
+            s = (self.q[:, h].double() @ k[:, kh].T * self.d ** -0.5).masked_fill(~seen, float("-inf"))
+            out.append(torch.softmax(s, -1) @ v[:, kh])
+        return torch.stack(out, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,requests,rows,heads,kv_heads,d", [(131072, 64, 1, 16, 8, 128), (131072, 32, 1, 16, 8, 256),
+                                                              (131072, 64, 1, 8, 8, 64), (65536, 96, 5, 12, 6, 128),
+                                                              (131072, 48, 17, 32, 8, 128)])
+def test_sums_do_not_drift_over_long_caches(n, requests, rows, heads, kv_heads, d, dtype):
+    st = Shared(n + d, n, requests, rows, heads, kv_heads, d, dtype)
+    assert bars.relative(st.run(), st.want()[None]) <= bars.relative_bar(dtype)
