@@ -8,9 +8,11 @@
 // code * 2^-24 (or code * 2^-20 for every second nibble), exact, with no conversion.  The query is
 // scaled by a power of two per column (its largest entry to [2^13, 2^14)) and by 1/16 where the
 // nibble brings 16, and rounded to F16 (exact for bf16 and f16 entries within 2^24 of the largest).
-// P * s is rounded to F16 once (bf16 calls: the output's own rounding is eight times as coarse), or kept
-// in two F16 parts with a second product (FINE, F16 calls: with one part the output's error was twice its
-// rounding's); m, sums and accumulators are f32.
+// P * s is rounded to F16 (h), once for bf16 calls.  Against the whole code that rounding would count
+// up to three times the value it stands for, since code * s and m nearly cancel; so the minima's sum takes
+// P (m + 7.5 s) - 7.5 h, and what h lost counts against code - 7.5, which is of the value's size: 1.68e-3 off where
+// the bf16 output's own rounding is 1.67e-3 (1.74e-3 without; 114 -> 117 us for 64 requests).  F16 calls keep P * s
+// in two F16 parts with a second product (FINE; 2.2e-4 off of 2.1e-4).  m, sums and accumulators are f32.
 //
 // The softmax reference of a column is kept so that P * s <= 2^15, whatever the values' magnitude:
 // it moves (one vote a step) only when a score or a step would pass that, with 2^4 to spare.
@@ -477,7 +479,8 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                         for (int rr = 0; rr < 2; rr++) {
                             const float2 vp = vpar[gi][rr][gr];
                             float a0 = p[2 * rr] * vp.x, a1 = p[2 * rr + 1] * vp.x;
-                            float b0 = p[2 * rr], b1 = p[2 * rr + 1], m0 = vp.y, m1 = vp.y;
+                            const float mid = FINE ? vp.y : fmaf(7.5f, vp.x, vp.y);
+                            float b0 = p[2 * rr], b1 = p[2 * rr + 1], m0 = mid, m1 = mid;
                             if constexpr (!FULL) {  // a key one row sees and another does not may hold NaN
                                 if (b0 == 0.0f) a0 = m0 = 0.0f;
                                 if (b1 == 0.0f) a1 = m1 = 0.0f;
@@ -485,11 +488,14 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                             mn[gr][nt][0] = fmaf(b0, m0, mn[gr][nt][0]);
                             mn[gr][nt][1] = fmaf(b1, m1, mn[gr][nt][1]);
                             const __half2 h2 = __floats2half2_rn(a0, a1);
+                            const float2 r2 = __half22float2(h2);
                             pb[gr][nt][rr] = movmatrix(*reinterpret_cast<const uint32_t*>(&h2));
                             if constexpr (FINE) {
-                                const float2 r2 = __half22float2(h2);
                                 const __half2 l2 = __floats2half2_rn(a0 - r2.x, a1 - r2.y);
                                 pl[gr][nt][rr] = movmatrix(*reinterpret_cast<const uint32_t*>(&l2));
+                            } else {
+                                mn[gr][nt][0] = fmaf(-7.5f, r2.x, mn[gr][nt][0]);
+                                mn[gr][nt][1] = fmaf(-7.5f, r2.y, mn[gr][nt][1]);
                             }
                         }
                 }

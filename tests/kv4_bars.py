@@ -14,7 +14,13 @@ counts: a zero query gives every visible key the same probability, and key p's v
     p // block of the head and 0 in the others, which the cache holds exactly; an output is then
     15/16 * (visible keys of the block) / (visible keys), whose products and sums are exact, so only the
     division and the output's rounding are off: (u + 2^-20) of it, where one key more or less is
-    1/block of it."""
+    1/block of it.
+
+beyond rounding: what an output is off by that its own rounding does not explain, over many outputs:
+    sqrt(error^2 - rounding^2) of their norms against the outputs'.  A probability times step of 11 bits is off
+    by 2.1e-4 (rms); where that counts against the value's own size it gives 2.1e-4 here.  64 normal channels span
+    about 4.8 deviations, 15 steps: against the whole code (0 to 15) it would be 2.6 times as much, 5.5e-4.
+    The bar is 3.2e-4, one and a half of the former."""
 
 import torch
 
@@ -51,3 +57,13 @@ def counts(n, rows, d, block, window=0, device="cpu"):
 def count_bar(want, dtype):
     """The allowed error of each output (a channel without visible keys is 0 exactly)."""
     return want * (UNIT[dtype] + 2.0 ** -20)
+
+
+BEYOND_BAR = 3.2e-4
+
+
+def beyond_rounding(got, want):
+    """sqrt(|error|^2 - |own rounding|^2) against |want|, over all outputs."""
+    error = (got.double() - want).norm()
+    own = (want.to(got.dtype).double() - want).norm()
+    return (error.square() - own.square()).clamp(min=0).sqrt().item() / want.norm().item()
