@@ -482,8 +482,8 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                             const float mid = FINE ? vp.y : fmaf(7.5f, vp.x, vp.y);
                             float b0 = p[2 * rr], b1 = p[2 * rr + 1], m0 = mid, m1 = mid;
                             if constexpr (!FULL) {  // a key one row sees and another does not may hold NaN
-                                if (b0 == 0.0f) a0 = m0 = 0.0f;
-                                if (b1 == 0.0f) a1 = m1 = 0.0f;
+                                if (x[gi][nt][2 * rr] == -CUDART_INF_F) a0 = m0 = 0.0f;
+                                if (x[gi][nt][2 * rr + 1] == -CUDART_INF_F) a1 = m1 = 0.0f;
                             }
                             mn[gr][nt][0] = fmaf(b0, m0, mn[gr][nt][0]);
                             mn[gr][nt][1] = fmaf(b1, m1, mn[gr][nt][1]);

@@ -70,3 +70,20 @@ def test_sums_do_not_drift_over_long_caches(n, requests, rows, heads, kv_heads, 
 def test_bf16_outputs_of_few_rows_are_off_by_little_more_than_their_rounding(rows, heads, kv_heads, d):
     st = Shared(rows + d, 6000, 2, rows, heads, kv_heads, d, torch.bfloat16)
     assert bars.beyond_rounding(st.run(), st.want()[None].expand(2, -1, -1, -1)) <= bars.BEYOND_BAR
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 3, 130])
+@pytest.mark.parametrize("at", [5, 40, 291])
+def test_a_nan_value_reaches_its_rows_however_little_it_weighs(d, n, at):
+    """Key `at` scores 8 * 8 * sqrt(d) below the others, so its probability is 0 in 32 bits; 0 * NaN is NaN."""
+    f = dict(generator=gen(d + n + at), device="cuda")
+    k, v = (torch.randn((300, 1, d), **f).to(torch.bfloat16) for _ in range(2))
+    k[at], v[at, 0, d - 1] = -8.0, float("nan")
+    cache = sx().Kv4Cache(19, 1, d, 16)
+    sx().kv4_write(cache, k, v, torch.arange(300, device="cuda"))
+    q = torch.full((n, 1, d), 8.0, dtype=torch.bfloat16, device="cuda")
+    got = sx().kv4_attention(q, cache, torch.arange(19, device="cuda", dtype=torch.int32)[None], i32([300]), i32([0, n]), n)[:, 0]
+    first = max(0, at - (300 - n))
+    assert torch.isnan(got[first:, d - 64:]).all()
+    assert torch.isfinite(got[:first]).all() and torch.isfinite(got[:, :d - 64]).all()
