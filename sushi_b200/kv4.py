@@ -5,11 +5,13 @@
     out = kv4_attention(q, cache, table, t.kv_lens, t.cu_q, max_q)
 
 The reference serves attention from its own host engine and has no counterpart of these calls; names,
-checks and errors are those of the rest of the package.  Everything is ordered on the current
-stream, allocates nothing but its outputs (and the attention's workspace, once a stream) and can be
-recorded in a CUDA graph.
+checks and errors are those of the rest of the package.  A call's tensors lie on one GPU, the
+cache's (SX_ERR_BAD_SHAPE otherwise).  Everything is ordered on that GPU's current stream, allocates
+nothing but its outputs (and the attention's workspace, once a stream) and can be recorded in a CUDA
+graph.
 """
 
+import contextlib
 import ctypes
 from typing import NamedTuple
 
@@ -21,9 +23,17 @@ from .exl3 import _DT, Exl3Error, _check, lib
 _I32, _I64, _U8 = torch.int32, torch.int64, torch.uint8
 
 
-def _stream(device):
-    """The current stream's handle on `device` (as an int: no Stream object a call)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _stream(gpu):
+    """The current stream's handle on GPU number `gpu` (as an int: no Stream object a call)."""
+    return torch._C._cuda_getCurrentRawStream(gpu)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _current(gpu):
+    """GPU number `gpu` as the current one, where launches and allocations go."""
+    return _HERE if torch._C._cuda_getDevice() == gpu else torch.cuda.device(gpu)
 
 
 class Kv4Cache:
@@ -40,9 +50,9 @@ class Kv4Cache:
             pool = torch.empty((self.pages, self.kv_heads, block), dtype=torch.uint8, device=device)
         elif pool.dtype != torch.uint8:
             raise Exl3Error(2)
-        elif pool.numel() != self.pages * self.kv_heads * block or not pool.is_contiguous() or not pool.is_cuda:
+        if pool.numel() != self.pages * self.kv_heads * block or not pool.is_contiguous() or not pool.is_cuda:
             raise Exl3Error(1)
-        self.pool = pool
+        self.pool, self.gpu = pool, pool.get_device()
         self._c = _lib.SxKv4(pool.data_ptr(), self.pages, self.kv_heads, self.head_dim, self.page_size)
         self._ref = ctypes.byref(self._c)
 
@@ -60,18 +70,18 @@ class BlockTables(NamedTuple):
     free_left: torch.Tensor  # [1] int32
 
 
-def _ints(t, n=None, dtype=_I32):
+def _ints(t, gpu, n=None, dtype=_I32):
     if t.dtype is not dtype:
         raise Exl3Error(2)
-    if not t.is_cuda or not t.is_contiguous() or (n is not None and t.numel() != n):
+    if t.get_device() != gpu or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise Exl3Error(1)
     return t.data_ptr()
 
 
-def _table(table, requests):
+def _table(table, gpu, requests):
     if table.dtype is not _I32:
         raise Exl3Error(2)
-    if not table.is_cuda or table.dim() != 2:
+    if table.get_device() != gpu or table.dim() != 2:
         raise Exl3Error(1)
     (rows, width), (stride, inner) = table.shape, table.stride()
     if rows != requests or width < 1 or (inner != 1 and width > 1):
@@ -85,26 +95,28 @@ def block_tables(ctx_lens, new_lens, table, free_pages, free_count, page_size: i
     new lengths [requests] int32 and the stack free_pages [n] int32 / free_count [1] int32.  The new
     stack height is `free_left` (negative: pages were short)."""
     requests = ctx_lens.numel()
-    c, n = _ints(ctx_lens), _ints(new_lens, requests)
-    t, width, stride = _table(table, requests)
-    f, fc = _ints(free_pages), _ints(free_count, 1)
+    gpu = max(ctx_lens.get_device(), 0)  # a host tensor (-1) is refused like one of another GPU
+    c, n = _ints(ctx_lens, gpu), _ints(new_lens, gpu, requests)
+    t, width, stride = _table(table, gpu, requests)
+    f, fc = _ints(free_pages, gpu), _ints(free_count, gpu, 1)
     tokens = int(tokens)
     if tokens < 0:
         raise Exl3Error(1)
-    # one buffer for the five outputs: slots (64-bit) first
-    buf = ctx_lens.new_empty(3 * tokens + 2 * requests + 2)
-    slots, positions, kv_lens, cu_q, left = buf.split_with_sizes([2 * tokens, tokens, requests, requests + 1, 1])
-    p = buf.data_ptr()
-    _check(lib().sx_block_tables(_stream(buf.device), c, n, requests, page_size, t, width, stride, f, fc, tokens,
-                                 p + 12 * tokens, p + 12 * tokens + 4 * requests, p, p + 8 * tokens,
-                                 p + 12 * tokens + 8 * requests + 4))
+    with _current(gpu):
+        # one buffer for the five outputs: slots (64-bit) first
+        buf = ctx_lens.new_empty(3 * tokens + 2 * requests + 2)
+        slots, positions, kv_lens, cu_q, left = buf.split_with_sizes([2 * tokens, tokens, requests, requests + 1, 1])
+        p = buf.data_ptr()
+        _check(lib().sx_block_tables(_stream(gpu), c, n, requests, page_size, t, width, stride, f, fc, tokens,
+                                     p + 12 * tokens, p + 12 * tokens + 4 * requests, p, p + 8 * tokens,
+                                     p + 12 * tokens + 8 * requests + 4))
     return BlockTables(kv_lens, cu_q, slots.view(_I64), positions, left)
 
 
-def _rows(x, heads, head_dim):
+def _rows(x, gpu, heads, head_dim):
     if x.dtype not in _DT:
         raise Exl3Error(2)
-    if not x.is_cuda or x.dim() != 3:
+    if x.get_device() != gpu or x.dim() != 3:
         raise Exl3Error(1)
     (_, h, d), (ts, hs, inner) = x.shape, x.stride()
     if h != heads or d != head_dim or inner != 1:
@@ -115,14 +127,16 @@ def _rows(x, heads, head_dim):
 def kv4_write(cache: Kv4Cache, k, v, slots):
     """sx_kv4_write: k and v [tokens, kv_heads, head_dim] (bf16/f16/f32; channels contiguous, any
     strides between tokens and heads) into the places slots [tokens] int64; -1 skips a token."""
-    kp, vp = _rows(k, cache.kv_heads, cache.head_dim), _rows(v, cache.kv_heads, cache.head_dim)
+    gpu = cache.gpu
+    kp, vp = _rows(k, gpu, cache.kv_heads, cache.head_dim), _rows(v, gpu, cache.kv_heads, cache.head_dim)
     if v.dtype != k.dtype:
         raise Exl3Error(2)
     if v.shape[0] != k.shape[0]:
         raise Exl3Error(1)
     tokens = k.shape[0]
-    s = _ints(slots, tokens, _I64)
-    _check(lib().sx_kv4_write(_stream(k.device), cache._ref, *kp, *vp, _DT[k.dtype], tokens, s))
+    s = _ints(slots, gpu, tokens, _I64)
+    with _current(gpu):
+        _check(lib().sx_kv4_write(_stream(gpu), cache._ref, *kp, *vp, _DT[k.dtype], tokens, s))
 
 
 def kv4_read(cache: Kv4Cache, slots, dtype=torch.bfloat16):
@@ -130,11 +144,13 @@ def kv4_read(cache: Kv4Cache, slots, dtype=torch.bfloat16):
     two [tokens, kv_heads, head_dim] tensors (zeros where a slot is -1)."""
     if dtype not in _DT:
         raise Exl3Error(2)
-    s = _ints(slots, dtype=_I64)
+    gpu = cache.gpu
+    s = _ints(slots, gpu, dtype=_I64)
     n = slots.numel()
-    kv = slots.new_empty((2, n, cache.kv_heads, cache.head_dim), dtype=dtype)
-    k, v = kv.unbind()
-    _check(lib().sx_kv4_read(_stream(kv.device), cache._ref, s, n, _DT[dtype], k.data_ptr(), v.data_ptr()))
+    with _current(gpu):
+        kv = slots.new_empty((2, n, cache.kv_heads, cache.head_dim), dtype=dtype)
+        k, v = kv.unbind()
+        _check(lib().sx_kv4_read(_stream(gpu), cache._ref, s, n, _DT[dtype], k.data_ptr(), v.data_ptr()))
     return k, v
 
 
@@ -167,19 +183,26 @@ def kv4_attention(q, cache: Kv4Cache, table, kv_lens, cu_q, max_q: int, scale=No
     if q.dim() != 3:
         raise Exl3Error(1)
     tokens, heads, _ = q.shape
-    qp, ts, hs = _rows(q, heads, cache.head_dim)
+    gpu = cache.gpu
+    qp, ts, hs = _rows(q, gpu, heads, cache.head_dim)
     requests = kv_lens.numel()
-    kl, cu = _ints(kv_lens), _ints(cu_q, requests + 1)
-    t, width, stride = _table(table, requests)
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+    kl, cu = _ints(kv_lens, gpu), _ints(cu_q, gpu, requests + 1)
+    t, width, stride = _table(table, gpu, requests)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.get_device() != gpu):
         raise Exl3Error(1)
-    L, st = lib(), _stream(q.device)
-    if workspace is None:
-        need = L.sx_kv4_attention_workspace_bytes(cache._ref, requests, tokens, heads, max_q)
-        workspace = _workspace(max(need, 16), q.device, st)
-    _check(L.sx_kv4_attention(st, cache._ref, qp, ts, hs, _DT[q.dtype], tokens, heads, cu, kl, t, requests, width, stride,
-                              max_q, cache.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-                              workspace.data_ptr(), workspace.numel()))
+    if workspace is not None:
+        if workspace.dtype is not _U8:
+            raise Exl3Error(2)
+        if workspace.get_device() != gpu or not workspace.is_contiguous():
+            raise Exl3Error(1)
+    with _current(gpu):
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        L, st = lib(), _stream(gpu)
+        if workspace is None:
+            need = L.sx_kv4_attention_workspace_bytes(cache._ref, requests, tokens, heads, max_q)
+            workspace = _workspace(max(need, 16), q.device, st)
+        _check(L.sx_kv4_attention(st, cache._ref, qp, ts, hs, _DT[q.dtype], tokens, heads, cu, kl, t, requests, width,
+                                  stride, max_q, cache.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
+                                  workspace.data_ptr(), workspace.numel()))
     return out
