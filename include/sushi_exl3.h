@@ -384,7 +384,8 @@ sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slot
  * multiple of kv_heads; scale finite; requests 1..16384; requests * kv_heads * table_width * page_size / 2 below 2^31
  * (and as many tiles of keys times blocks of rows, where rows are many), else SX_ERR_BAD_SHAPE.
  * workspace: sx_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned; it keeps nothing between
- * calls, but calls that may run at the same time need their own. */
+ * calls, but calls that may run at the same time need their own.  So do calls of two host threads on one
+ * stream: a call is several launches, and another call's between them would overwrite what they pass on. */
 size_t sx_kv4_attention_workspace_bytes(const sx_kv4* cache, int32_t requests, int32_t tokens, int32_t heads,
                                         int32_t max_q);
 sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q, int64_t q_token_stride,

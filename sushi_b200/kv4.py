@@ -13,6 +13,7 @@ graph.
 
 import contextlib
 import ctypes
+import threading
 from typing import NamedTuple
 
 import torch
@@ -158,18 +159,21 @@ def kv4_attention_workspace_bytes(cache: Kv4Cache, requests: int, tokens: int, h
     return lib().sx_kv4_attention_workspace_bytes(cache._ref, int(requests), int(tokens), int(heads), int(max_q))
 
 
-_WS = {}
+class _Kept:
+    """A stream's workspace, kept for its next calls.  A call is several launches, the later ones reading what
+    the first left in the workspace: `lock` keeps another host thread's launches on the stream from coming
+    between them."""
+
+    def __init__(self):
+        self.lock, self.buffer = threading.Lock(), None
+
+    def grown(self, nbytes, device):
+        if self.buffer is None or self.buffer.numel() < nbytes:
+            self.buffer = torch.empty(nbytes, dtype=_U8, device=device)
+        return self.buffer
 
 
-def _workspace(nbytes, device, stream):
-    """The workspace of a stream, kept for its next calls; inside a graph recording one of the graph's own."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=_U8, device=device)
-    key = (device.index, stream)
-    ws = _WS.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = _WS[key] = torch.empty(nbytes, dtype=_U8, device=device)
-    return ws
+_WS = {}  # (GPU, stream) -> _Kept
 
 
 def kv4_attention(q, cache: Kv4Cache, table, kv_lens, cu_q, max_q: int, scale=None, window: int = 0, out=None,
@@ -179,7 +183,8 @@ def kv4_attention(q, cache: Kv4Cache, table, kv_lens, cu_q, max_q: int, scale=No
     of `table` [requests, width] names, the step's own last; causal, with a sliding window of
     `window` positions when it is positive.  scale: head_dim**-0.5 when None.  out: an optional
     contiguous tensor of q's shape and dtype.  workspace: an optional uint8 tensor of
-    kv4_attention_workspace_bytes(...) bytes, for the calls of one stream."""
+    kv4_attention_workspace_bytes(...) bytes, for the calls of one stream by one host thread (without
+    it, several threads may call on one stream)."""
     if q.dim() != 3:
         raise Exl3Error(1)
     tokens, heads, _ = q.shape
@@ -198,11 +203,18 @@ def kv4_attention(q, cache: Kv4Cache, table, kv_lens, cu_q, max_q: int, scale=No
     with _current(gpu):
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        L, st = lib(), _stream(gpu)
+        L, st, lock = lib(), _stream(gpu), _HERE
         if workspace is None:
-            need = L.sx_kv4_attention_workspace_bytes(cache._ref, requests, tokens, heads, max_q)
-            workspace = _workspace(max(need, 16), q.device, st)
-        _check(L.sx_kv4_attention(st, cache._ref, qp, ts, hs, _DT[q.dtype], tokens, heads, cu, kl, t, requests, width,
-                                  stride, max_q, cache.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-                                  workspace.data_ptr(), workspace.numel()))
+            need = max(L.sx_kv4_attention_workspace_bytes(cache._ref, requests, tokens, heads, max_q), 16)
+            if torch.cuda.is_current_stream_capturing():
+                workspace = torch.empty(need, dtype=_U8, device=q.device)  # the recorded graph's own
+            else:
+                kept = _WS.get((gpu, st)) or _WS.setdefault((gpu, st), _Kept())
+                lock = kept.lock
+        with lock:
+            if lock is not _HERE:
+                workspace = kept.grown(need, q.device)
+            _check(L.sx_kv4_attention(st, cache._ref, qp, ts, hs, _DT[q.dtype], tokens, heads, cu, kl, t, requests, width,
+                                      stride, max_q, cache.head_dim ** -0.5 if scale is None else scale, window,
+                                      out.data_ptr(), workspace.data_ptr(), workspace.numel()))
     return out

@@ -1,5 +1,7 @@
 """Attention over long caches, held to bars that a lost key or a drifting sum breaks (tests/kv4_bars.py)."""
 
+import threading
+
 import pytest
 import torch
 
@@ -87,3 +89,21 @@ def test_a_nan_value_reaches_its_rows_however_little_it_weighs(d, n, at):
     first = max(0, at - (300 - n))
     assert torch.isnan(got[first:, d - 64:]).all()
     assert torch.isfinite(got[:first]).all() and torch.isfinite(got[:, :d - 64]).all()
+
+
+def test_two_host_threads_on_one_stream():
+    """Long caches whose units are split over the CTAs and joined, from two threads at once on the default
+    stream: the bits of the calls one after another."""
+    cases = [Shared(51, 30000, 1, 1, 16, 2, 128, torch.bfloat16), Shared(52, 20000, 2, 40, 16, 2, 128, torch.bfloat16)]
+    want = [c.run() for c in cases]
+    got, start = [[], []], threading.Barrier(2)
+
+    def thread(i):
+        start.wait()
+        got[i] = [cases[i].run() for _ in range(60)]
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for i in range(2):
+        assert len(got[i]) == 60 and all(torch.equal(x, want[i]) for x in got[i])

@@ -2,6 +2,8 @@
 a GPU, and a library that records its calls."""
 
 import contextlib
+import threading
+import time
 
 import pytest
 import torch
@@ -112,3 +114,32 @@ def test_a_call_runs_on_its_tensors_gpu(rec, monkeypatch, call):
 def test_a_cache_on_the_host_is_refused():
     with pytest.raises(Exl3Error, match="SX_ERR_BAD_SHAPE"):
         kv4.Kv4Cache(3, 2, 64, 16, device="cpu")
+
+
+def test_calls_of_two_threads_on_one_stream_do_not_share_a_workspace_at_a_time(rec, monkeypatch):
+    """A call is several launches that pass partial results through the workspace: no other call may be
+    under way with it."""
+    c, busy, clashes = cache(rec, monkeypatch), set(), []
+
+    def launches(*args):
+        ws = args[-2]
+        clashes.extend([ws] if ws in busy else [])
+        busy.add(ws)
+        time.sleep(0.02)
+        busy.discard(ws)
+        return 0
+
+    rec.sx_kv4_attention = launches
+    start = threading.Barrier(4)
+
+    def thread():
+        t = tensors()
+        t["q"].device = torch.device("cpu")
+        start.wait()
+        for _ in range(3):
+            kv4.kv4_attention(t["q"], c, t["table"], t["kv_lens"], t["cu_q"], 1, out=t["out"])
+
+    threads = [threading.Thread(target=thread) for _ in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not clashes
