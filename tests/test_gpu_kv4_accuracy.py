@@ -7,6 +7,7 @@ import torch
 
 import kv4_bars as bars
 import kv4_ref as ref
+from test_gpu_kv4 import Step
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +108,86 @@ def test_two_host_threads_on_one_stream():
     [t.join() for t in threads]
     for i in range(2):
         assert len(got[i]) == 60 and all(torch.equal(x, want[i]) for x in got[i])
+
+
+# ------------------------------------------------------------------ every key counts, once
+class Centred(Step):
+    """A step whose values have no common mean, so that an output shows its keys and not the mean."""
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.v = (self.v.float() - 0.5).to(self.dtype)
+        sx().kv4_write(self.cache, self.k, self.v, self.slots)
+
+
+class Counted(Step):
+    """A step of the count statement: zero queries, and values that say which block of keys they are of."""
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.q.zero_()
+        self.blocks, v = [], []
+        for n, _ in self.lens:
+            x, block = bars.count_values(max(n, 1), self.d, "cuda")
+            v.append(x[:n])
+            self.blocks.append(block)
+        v = torch.cat(v)[:, None].expand(-1, self.cache.kv_heads, -1).to(self.dtype)
+        if len(v):
+            sx().kv4_write(self.cache, self.k, v, self.slots)
+
+    def check(self, got):
+        row = 0
+        for (n, r), block in zip(self.lens, self.blocks):
+            if r and n >= r:
+                assert block * (bars.UNIT[self.dtype] + 2.0 ** -20) < 1  # one key is more than the bar
+                want = bars.counts(n, r, self.d, block, self.window, "cuda")[:, None]
+                err = (got[row:row + r].double() - want).abs()
+                assert (err <= bars.count_bar(want, self.dtype)).all(), (n, r, (err - bars.count_bar(want, self.dtype)).max().item())
+            row += r
+
+
+LONG = {
+    "one": [(20000, 1)],
+    "ragged": [(9000, 1), (3, 1), (4100, 1)],
+    "draft": [(12000, 3), (2, 2), (5000, 8)],
+    "chunk": [(8200, 70), (100, 1)],
+    "mixed": [(5000, 1), (6000, 130), (4321, 5), (2500, 300), (7000, 1)],
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens", list(LONG))
+@pytest.mark.parametrize("d,heads,kv_heads,page", [(64, 8, 2, 16), (128, 8, 1, 64), (128, 16, 8, 32), (256, 4, 2, 64)])
+def test_long_caches_within_the_relative_bar(d, heads, kv_heads, page, lens, dtype):
+    st = Centred(61 + d, d, dtype, heads, kv_heads, page, LONG[lens])
+    got, (want, _) = st.run(), st.want()
+    row = 0
+    for n, r in st.lens:
+        if n >= 1000:
+            assert bars.relative(got[row:row + r], want[row:row + r]) <= bars.relative_bar(dtype), (n, r)
+        row += r
+
+
+@pytest.mark.parametrize("lens", list(LONG))
+@pytest.mark.parametrize("window", [0, 1, 100, 1000, 4099])
+@pytest.mark.parametrize("d,heads,kv_heads,page", [(64, 8, 2, 16), (128, 1, 1, 64), (128, 40, 1, 16), (128, 16, 8, 256), (256, 4, 2, 32)])
+def test_long_caches_count_every_key_once(d, heads, kv_heads, page, window, lens):
+    st = Counted(67 + d, d, torch.float16, heads, kv_heads, page, LONG[lens], window)
+    st.check(st.run())
+
+
+@pytest.mark.parametrize("lens", [[(131071, 1)], [(100003, 2), (60000, 1)], [(99991, 40)]])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 1), (16, 8)])
+def test_the_longest_caches_count_every_key_once(heads, kv_heads, lens):
+    st = Counted(71, 128, torch.float16, heads, kv_heads, 64, lens)
+    st.check(st.run())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 2, 7, 33, 150])
+def test_short_caches_count_every_key_once(rows, dtype, d):
+    """Lengths around every granule, step and tile edge."""
+    edges = sorted({max(rows, e + o) for e in (16, 32, 64, 128, 256, 384, 512) for o in (-1, 0, 1, 7)})
+    st = Counted(73 + rows, d, dtype, 6, 2, 16, [(n, rows) for n in edges])
+    st.check(st.run())
