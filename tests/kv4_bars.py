@@ -45,13 +45,18 @@ def count_values(n, d, device="cpu"):
     return v, block
 
 
-def counts(n, rows, d, block, window=0, device="cpu"):
-    """The count statement's outputs [rows, d] (f64) of the last `rows` positions of n keys."""
-    pos = torch.arange(n - rows, n, device=device)[:, None].double()
+def counts_at(pos, d, block, window=0):
+    """The count statement's outputs [rows, d] (f64) of rows at positions `pos` (0 of a row before position 0)."""
+    pos = pos[:, None].double()
     low = (pos - window + 1).clamp(min=0) if window else torch.zeros_like(pos)
-    first = torch.arange(d, device=device)[None, :].double() * block
+    first = torch.arange(d, device=pos.device)[None, :].double() * block
     inside = (torch.minimum(pos + 1, first + block) - torch.maximum(low, first)).clamp(min=0)
-    return 15.0 / 16.0 * inside / (pos - low + 1)
+    return 15.0 / 16.0 * inside / (pos - low + 1).clamp(min=1)
+
+
+def counts(n, rows, d, block, window=0, device="cpu"):
+    """Those of the last `rows` positions of n keys."""
+    return counts_at(torch.arange(n - rows, n, device=device), d, block, window)
 
 
 def count_bar(want, dtype):

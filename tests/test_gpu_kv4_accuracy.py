@@ -191,3 +191,33 @@ def test_short_caches_count_every_key_once(rows, dtype, d):
     edges = sorted({max(rows, e + o) for e in (16, 32, 64, 128, 256, 384, 512) for o in (-1, 0, 1, 7)})
     st = Counted(73 + rows, d, dtype, 6, 2, 16, [(n, rows) for n in edges])
     st.check(st.run())
+
+
+# ------------------------------------------------------------------ many requests
+@pytest.mark.parametrize("requests", [64, 65, 129, 513, 1025, 16384])
+@pytest.mark.parametrize("d,heads,kv_heads,chunks", [(64, 2, 1, {}), (128, 8, 2, {0: 70, 63: 33, -1: 200}), (256, 16, 1, {7: 5, -2: 90})])
+@pytest.mark.parametrize("window", [0, 37])
+def test_many_requests_count_every_key_once(requests, d, heads, kv_heads, chunks, window):
+    """Ragged requests over one shared row of pages, some without keys or rows, a few with many rows."""
+    n, page, g = 400, 16, gen(requests + d)
+    lens = torch.randint(0, n + 1, (requests,), generator=g, device="cuda", dtype=torch.int32)
+    rows = (torch.rand((requests,), generator=g, device="cuda") < 0.9).int()
+    for at, r in chunks.items():
+        rows[at], lens[at] = r, 250
+    cu = torch.cat([i32([0]), torch.cumsum(rows, 0, dtype=torch.int32)])
+    cache = sx().Kv4Cache(n // page, kv_heads, d, page)
+    v, block = bars.count_values(n, d, "cuda")
+    k = torch.randn((n, kv_heads, d), generator=g, device="cuda").half()
+    ids = torch.randperm(n // page, generator=g, device="cuda")
+    pos = torch.arange(n, device="cuda")
+    sx().kv4_write(cache, k, v[:, None].expand(-1, kv_heads, -1).half(), ids[pos // page] * page + pos % page)
+    tokens = int(cu[-1])
+    q = torch.zeros((tokens + 3, heads, d), dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, 7.0)
+    sx().kv4_attention(q, cache, ids.int()[None].repeat(requests, 1), lens, cu, max([1, *chunks.values()]), window=window, out=out)
+    b = torch.repeat_interleave(torch.arange(requests, device="cuda"), rows.long())
+    at = lens.long()[b] - rows.long()[b] + torch.arange(tokens, device="cuda") - cu.long()[b]
+    want = bars.counts_at(at, d, block, window)
+    assert ((out[:tokens].double() - want[:, None]).abs() <= bars.count_bar(want, torch.float16)[:, None]).all()
+    assert not out[tokens:].any()
+    assert sx().device_error() == 0
