@@ -381,7 +381,7 @@ sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slot
  * Positions whose page id is outside the pool, or past table_width pages, count as unseen.
  * q [tokens][heads][head_dim] with strides in elements, channels contiguous; out contiguous and
  * 16-byte aligned; both of `dtype`, BF16 or F16 (SX_ERR_BAD_DTYPE for F32: the products take 16-bit operands).  heads is a
- * multiple of kv_heads; scale finite; requests 1..16384; requests * kv_heads * table_width * page_size / 2 below 2^31
+ * multiple of kv_heads; |scale| < 2^100; requests 1..16384; requests * kv_heads * table_width * page_size / 2 below 2^31
  * (and as many tiles of keys times blocks of rows, where rows are many), else SX_ERR_BAD_SHAPE.
  * workspace: sx_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned; it keeps nothing between
  * calls, but calls that may run at the same time need their own.  So do calls of two host threads on one

@@ -55,7 +55,7 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     if (st) return st;
     if (dtype != SX_DT_F16 && dtype != SX_DT_BF16) return SX_ERR_BAD_DTYPE;
     if (tokens < 0 || heads < 1 || heads % cache->kv_heads || requests < 1 || requests > kKvMostRequests || table_width < 1 ||
-        table_stride < table_width || max_q < 1 || window < 0 || !std::isfinite(scale))
+        table_stride < table_width || max_q < 1 || window < 0 || !(std::fabs(scale) < 0x1p100f))
         return SX_ERR_BAD_SHAPE;
     // the work lists count steps (of 16 tokens at the smallest; tiles of keys) in 32 bits
     const long long most = most_pairs(cache, heads, max_q);

@@ -45,6 +45,21 @@ __device__ __forceinline__ Kv4Request kv4_request(const Kv4AttnArgs& a, int b) {
     return r;
 }
 
+// A softmax reference before any score; below every score (|score| log2(e) <= 2^126, see kv4_most_scale).
+constexpr float kNoScore = -3.0e38f;
+
+// The factor from a product of prepared operands (below 2^`bits`) to a score, kept so that scores are finite: a
+// score's 24 bits then stand for differences of 2^40 and more, so the softmax is its limit already.
+__device__ __forceinline__ float kv4_most_scale(float c, int bits) {
+    const float most = __uint_as_float((uint32_t)(127 + 126 - bits) << 23);
+    return fminf(fmaxf(c, -most), most);
+}
+
+// 2^k that brings a query row's largest entry into [2^13, 2^14); 1 for a row of zeros or without a finite largest.
+__device__ __forceinline__ int query_scale(float top) {
+    return top > 0.0f && top <= 3.402823466e38f ? min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -120), 120) : 0;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -33,7 +33,7 @@ __device__ __forceinline__ void join_column(const Kv4AttnArgs& a, const Kv4Reque
     constexpr int J = 64 / E < 16 ? 64 / E : 16;
     float y[J][E], mw;
     auto fetch = [&](int k0) {
-        mw = lane < J && k0 + lane * parts < shares ? __ldcg(share(k0 + lane * parts) + kStRows * D + 2 * c) : -1.0e30f;
+        mw = lane < J && k0 + lane * parts < shares ? __ldcg(share(k0 + lane * parts) + kStRows * D + 2 * c) : kNoScore;
 #pragma unroll
         for (int j = 0; j < J; j++) {
 #pragma unroll
@@ -54,7 +54,7 @@ __device__ __forceinline__ void join_column(const Kv4AttnArgs& a, const Kv4Reque
         }
     };
     fetch(part);
-    float top = -1.0e30f, ls = 0.0f;
+    float top = kNoScore, ls = 0.0f;
 #pragma unroll 2
     for (int k = lane; k < shares; k += 32) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(share(k) + kStRows * D + 2 * c));
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) kv4_join_tile_kernel(Kv4AttnA
         const int c = tid / PARTS, part = tid % PARTS;
         constexpr int H = kJoinShares / PARTS;
         float held[H];
-        float top = -1.0e30f, ls = 0.0f;
+        float top = kNoScore, ls = 0.0f;
         auto take = [&](const float2& ml) {
             const float up = fmaxf(top, ml.x);
             ls = fmaf(ls, ex2(top - up), ml.y * ex2(ml.x - up));
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) kv4_join_tile_kernel(Kv4AttnA
 #pragma unroll
         for (int i = 0; i < H; i++) {
             const int k = part + i * PARTS;
-            ml[i] = c < rows && k < shares ? __ldcg(reinterpret_cast<const float2*>(share(k) + ml_at + 2 * c)) : make_float2(-1.0e30f, 0.0f);
+            ml[i] = c < rows && k < shares ? __ldcg(reinterpret_cast<const float2*>(share(k) + ml_at + 2 * c)) : make_float2(kNoScore, 0.0f);
         }
 #pragma unroll
         for (int i = 0; i < H; i++) {

@@ -275,9 +275,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
 #pragma unroll
             for (int e = 0; e < E; e++) top = fmaxf(top, fabsf(x[w][e]));
             top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));  // entries of no sign order as integers
-            // 2^k with top * 2^k in [2^13, 2^14); 1 for a column of zeros or without a finite maximum
-            int k = 0;
-            if (top > 0.0f && top < 3.0e38f) k = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -120), 120);
+            const int k = query_scale(top);
             const float up = __uint_as_float((uint32_t)(k + 127) << 23);
             float sum = 0.0f;
 #pragma unroll
@@ -294,7 +292,8 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
 #pragma unroll
             for (int m = 32 / G / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
             if (lane % (32 / G) == 0) qs_sm[c * G + lane / (32 / G)] = sum * 5.9604644775390625e-08f;  // 2^-24
-            if (lane == 0) ch_sm[c] = a.scale_log2 * 16777216.0f * __uint_as_float((uint32_t)(127 - k) << 23);
+            // (codes * s and m below 2^16, the query below 2^14, 2^8 channels, 2^-24)
+            if (lane == 0) ch_sm[c] = kv4_most_scale(a.scale_log2 * 16777216.0f * __uint_as_float((uint32_t)(127 - k) << 23), 16);
         }
         __syncthreads();
         float qs[NT][2][G], chs[NT][2];
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 l[nt][j] = 0.0f;
-                mref[nt][j] = thr[nt][j] = -1.0e30f;
+                mref[nt][j] = thr[nt][j] = kNoScore;
 #pragma unroll
                 for (int gr = 0; gr < G; gr++) mn[gr][nt][j] = 0.0f;
             }

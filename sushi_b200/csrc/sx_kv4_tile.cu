@@ -419,12 +419,13 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                     for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
                 }
             }
-            int k2 = 0;
-            if (top > 0.0f && top < 3.0e38f) k2 = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -120), 120);
+            const int k2 = query_scale(top);
             // a negative scale goes into the query's sign, so that c >= 0 below
             const float up = copysignf(__uint_as_float((uint32_t)(k2 + 127) << 23), a.scale_log2);
-            // (a scale of 0 keeps c above 0: -inf c is then -inf, and what is left of the scores adds nothing)
-            const float c = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k2) << 23), 1.0e-30f);
+            // (a scale of 0 keeps c above 0: -inf c is then -inf, and what is left of the scores adds nothing; keys below
+            // 2^16, the query below 2^14, 2^8 channels)
+            float c = fmaxf(kv4_most_scale(fabsf(a.scale_log2) * __uint_as_float((uint32_t)(127 - k2) << 23), 38), 1.0e-30f);
+            volatile float c_first = c;  // not worth a register: read once, after the tiles
 #pragma unroll
             for (int b = 0; b < D / 64; b++) {
                 if (!HOLD) load_q(b * 64, qw[0]);
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
             // tiles of keys that start at or after full_lo and end by full_hi are seen whole by every pair
             const int full_hi = min(r.hi, r.pos0 + un.e0 / a.group + 1) - NK;
             const int full_lo = a.window > 0 ? r.pos0 + (un.e0 + un.rows - 1) / a.group - a.window + 1 : 0;
-            float mref = -1.0e30f, l = 0.0f;
+            float mref = kNoScore, l = 0.0f;
             uint32_t bad = 0;  // groups in which the row sees a NaN value
             for (int j = 0; tile_live && j < n; j++, turns++) {
                 const int bi = MT == 2 ? mt : (int)(turns & 1);
@@ -510,7 +511,13 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                 }
                 const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
                 if (__any_sync(0xffffffffu, mx > mref + 15.0f)) {
-                    const float moved = fmaxf(mref, mx - 7.0f);
+                    // c S - mref, in one rounding, is off by mref's own: past 2^22 the row's c shrinks by a power of two.
+                    // Two scores of 11-bit operands that differ at all then still differ by 2^10.
+                    float size = 1.0f;
+                    if (fabsf(mx) > 4194304.0f && mx > kNoScore) size = __uint_as_float((275u << 23) - (__float_as_uint(mx) & 0x7f800000u));
+                    c *= size;
+                    mref *= size;
+                    const float moved = fmaxf(mref, mx * size - 7.0f);
                     const float f = ex2(mref - moved);
                     mref = moved;
                     l *= f;
@@ -615,7 +622,7 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
                 __syncwarp();
                 tc_fence_before();  // the next unit's first product overwrites O after the next arrival
                 if (!whole && live)
-                    __stcg(reinterpret_cast<float2*>(slot + kv4_tile_rows(D) * D + 2 * e), make_float2(mref, l));
+                    __stcg(reinterpret_cast<float2*>(slot + kv4_tile_rows(D) * D + 2 * e), make_float2(mref * (c_first / c), l));
             }
             pos = seg_end;
         }

@@ -221,3 +221,35 @@ def test_many_requests_count_every_key_once(requests, d, heads, kv_heads, chunks
     assert ((out[:tokens].double() - want[:, None]).abs() <= bars.count_bar(want, torch.float16)[:, None]).all()
     assert not out[tokens:].any()
     assert sx().device_error() == 0
+
+
+# ------------------------------------------------------------------ scores of any finite magnitude
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n,rows", [(300, 1), (300, 3), (700, 130), (20000, 1), (9000, 40)])
+@pytest.mark.parametrize("q,scale", [(1e4, None), (1e7, None), (1e20, None), (1e36, None), (3.3e38, None), (-1e30, None), (-3.3e38, -1.0),
+                                     (1.0, 1e30), (1e-3, -1e20), (1e-38, None), (1e-38, 1e20), (3e38, 0.0)])
+def test_scores_of_any_finite_magnitude(n, rows, d, q, scale):
+    """One key points along the query, one against it, ten times as far as any other: the softmax is one of
+    them, or the mean where scores are nothing."""
+    f = dict(generator=gen(n + rows + d), device="cuda")
+    k = (torch.rand((n, 1, d), **f) * 0.2 - 0.1).to(torch.bfloat16)
+    v = torch.randn((n, 1, d), **f).to(torch.bfloat16)
+    first = n - rows
+    at, against = first // 3, first // 2  # seen by every row
+    k[at], k[against] = 1.0, -1.0
+    page = 64
+    pages = -(-n // page)
+    cache = sx().Kv4Cache(pages, 1, d, page)
+    sx().kv4_write(cache, k, v, torch.arange(n, device="cuda"))
+    qs = torch.full((rows, 6, d), q, dtype=torch.bfloat16, device="cuda")
+    got = sx().kv4_attention(qs, cache, torch.arange(pages, device="cuda", dtype=torch.int32)[None], i32([n]), i32([0, rows]), rows,
+                             scale=scale)
+    values = ref.held(v)[0][:, 0]
+    s = (d ** -0.5 if scale is None else scale) * float(qs[0, 0, 0]) * d
+    if abs(s) > 1e3:
+        want = values[at if s > 0 else against].expand(rows, 6, d)
+        assert ((got.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -10) * want.abs().max()).all()
+    else:
+        want = (values.cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None])[first:, None]
+        assert abs(s) < 1e-10 and bars.relative(got, want) <= bars.relative_bar(torch.bfloat16)
+    assert sx().device_error() == 0

@@ -143,3 +143,10 @@ def test_calls_of_two_threads_on_one_stream_do_not_share_a_workspace_at_a_time(r
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not clashes
+
+
+@pytest.mark.parametrize("scale,want", [(2.0 ** 100, "SX_ERR_BAD_SHAPE"), (-3e38, "SX_ERR_BAD_SHAPE"), (2.0 ** 99, "SX_OK"), (0.0, "SX_OK")])
+def test_scales(scale, want):
+    from test_kv4_host import attention
+
+    assert attention(kv4._lib.load(), tokens=0, scale=scale) == want
