@@ -171,15 +171,16 @@ __device__ __forceinline__ int block_scan(int v, int* red, int& before) {
     return all;
 }
 
-// The list's length by steps(b) of every request, W warps together; n0 is steps(threadIdx.x).
+// The list's length by steps(b) of every request, W warps together; n0 is steps(threadIdx.x).  `mark`, which
+// steps() may set, is then true for every thread if it was for one.
 template <int W, typename F>
-__device__ __forceinline__ int list_total(int requests, int* red, int& n0, F steps) {
+__device__ __forceinline__ int list_total(int requests, int* red, int& n0, bool& mark, F steps) {
     n0 = (int)threadIdx.x < requests ? steps((int)threadIdx.x) : 0;
     int v = n0;
     for (int b = threadIdx.x + W * 32; b < requests; b += W * 32) v += steps(b);
     v = __reduce_add_sync(0xffffffffu, v);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
+    mark = __syncthreads_or(mark);
     int all = 0;
 #pragma unroll
     for (int w = 0; w < W; w++) all += red[w];
@@ -204,10 +205,11 @@ __device__ __forceinline__ void list_find(int requests, int* red, int* pick, int
 }
 
 // The tile kernel's list, W warps together: every request's tiles (over one key head), by a warp a request
-// where requests are few (their blocks are many then), else by a thread; `each` sees every unit once.
+// where requests are few (their blocks are many then), else by a thread; `each` sees every unit once, and may set
+// `mark` (as list_total's steps).
 constexpr int kTlFew = 64;
 template <int D, int W, typename F>
-__device__ __forceinline__ int tile_list_total(const Kv4AttnArgs& a, int* red, int* few, int& n0, F each) {
+__device__ __forceinline__ int tile_list_total(const Kv4AttnArgs& a, int* red, int* few, int& n0, bool& mark, F each) {
     auto request = [&](int b, int u0, int du) {
         const Kv4Request r = kv4_request(a, b);
         const int blocks = tile_blocks<D>(a, r);
@@ -225,9 +227,9 @@ __device__ __forceinline__ int tile_list_total(const Kv4AttnArgs& a, int* red, i
             if ((threadIdx.x & 31) == 0) few[b] = n * a.kv_heads;
         }
         __syncthreads();
-        return list_total<W>(a.requests, red, n0, [&](int b) { return few[b]; });
+        return list_total<W>(a.requests, red, n0, mark, [&](int b) { return few[b]; });
     }
-    return list_total<W>(a.requests, red, n0, [&](int b) { return request(b, 0, 1) * a.kv_heads; });
+    return list_total<W>(a.requests, red, n0, mark, [&](int b) { return request(b, 0, 1) * a.kv_heads; });
 }
 
 // The unit that holds step `at` of the list: request pick[0], block pick[2], key head pick[4]; its first

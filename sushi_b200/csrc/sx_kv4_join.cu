@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(kJoinThreads, 2) kv4_join_tile_kernel(Kv4AttnA
     const int cut = (int)blockIdx.x / TG + 1, row0 = (int)blockIdx.x % TG * ROWS, tid = threadIdx.x;
     pdl_release();
     int n0;
-    const int total = tile_list_total<D, kJoinWarps>(a, red, few, n0, [](int, const Kv4Request&, const TileUnit&, int) {});
+    bool mark = false;
+    const int total = tile_list_total<D, kJoinWarps>(a, red, few, n0, mark, [](int, const Kv4Request&, const TileUnit&, int) {});
     const RunCut run(total, tile_grid);
     if (total == 0 || cut >= run.ctas) {  // a CTA with nothing to join waits too: this grid's end stands for the whole call's
         pdl_wait();

@@ -98,6 +98,44 @@ __device__ __forceinline__ void tile_seek(const Kv4AttnArgs& a, TileCursor& c, i
     }
 }
 
+// Zeros for the blocks of this CTA that see no key, a warp a block: its lanes look for them in 32 requests at a time.
+template <int D, int W>
+__device__ __forceinline__ void tile_zeros(const Kv4AttnArgs& a) {
+    const int lane = threadIdx.x & 31, grid = gridDim.x;
+    for (int b0 = (int)(threadIdx.x >> 5) * 32; b0 < a.requests; b0 += W * 32) {
+        const int b = b0 + lane;
+        Kv4Request r = {};
+        int blocks = 0;
+        if (b < a.requests) {
+            r = kv4_request(a, b);
+            blocks = tile_blocks<D>(a, r);
+        }
+        // the first block u with (b + u) % grid this CTA
+        for (int u = ((int)blockIdx.x - b % grid + grid) % grid; __any_sync(0xffffffffu, u < blocks); u += grid) {
+            TileUnit t = {};
+            t.n = 1;
+            if (u < blocks) t = tile_unit<D>(a, r, u);
+            for (unsigned m = __ballot_sync(0xffffffffu, t.n == 0); m; m &= m - 1) {
+                const int from = __ffs(m) - 1;
+                const int q0 = __shfl_sync(0xffffffffu, r.q0, from), e0 = __shfl_sync(0xffffffffu, t.e0, from),
+                          rows = __shfl_sync(0xffffffffu, t.rows, from);
+                // whole tokens [t0, t1) are one piece; of the tokens at the ends, pairs [e0, t0 group) and [t1 group, e1)
+                const int e1 = e0 + rows, t1 = e1 / a.group, t0 = min((e0 + a.group - 1) / a.group, t1);
+                uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)q0 * a.heads * D);
+                const size_t row = (size_t)a.heads * (D / 8);
+                for (size_t i = t0 * row + lane; i < t1 * row; i += 32) o[i] = make_uint4(0, 0, 0, 0);
+                auto pairs = [&](int first, int last) {
+                    for (int h = 0; h < a.kv_heads; h++)
+                        for (int e = first; e < last; e++)
+                            if (lane < D / 8) o[e / a.group * row + (h * a.group + e % a.group) * (D / 8) + lane] = make_uint4(0, 0, 0, 0);
+                };
+                pairs(e0, min(e1, max(t0 * a.group, e0)));
+                pairs(max(t1 * a.group, e0), e1);
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void tc_mma_ts_f16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                               uint32_t accumulate) {
     asm volatile(
@@ -279,7 +317,7 @@ __device__ __forceinline__ void widen_values(const uint8_t* gran, int live, int 
 }
 
 template <int D>
-__global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4AttnArgs a) {
+__global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using L = TileLayout<D>;
     constexpr int G = L::G, MT = L::MT, NK = L::NK, NG = L::NG;
     extern __shared__ uint8_t smem_raw[];
@@ -305,22 +343,18 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(Kv4
         fence_mbar_init();
     }
 
-    // ---------------- the list's length; rows of blocks that see no key are zeroed here
+    // ---------------- the list's length; blocks that see no key are zeroed here, by CTA (request + block) % grid
     const size_t head_row = (size_t)a.heads * D;
     pdl_release();
     constexpr int W = L::THREADS / 32;
-    int n0;
-    const int total = tile_list_total<D, W>(a, red, few, n0, [&](int b, const Kv4Request& r, const TileUnit& t, int u) {
-        if (t.n == 0 && (b + u) % (int)gridDim.x == (int)blockIdx.x)
-            for (int h = 0; h < a.kv_heads; h++)
-                for (int e = t.e0; e < t.e0 + t.rows; e++) {
-                    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + e / a.group) * head_row +
-                                                        (size_t)(h * a.group + e % a.group) * D);
-                    for (int i = 0; i < D / 8; i++) o[i] = make_uint4(0, 0, 0, 0);
-                }
-    });
-    const RunCut run(total, gridDim.x);
     const int cta = blockIdx.x;
+    int n0;
+    bool zeros = false;
+    const int total = tile_list_total<D, W>(a, red, few, n0, zeros, [&](int b, const Kv4Request&, const TileUnit& t, int u) {
+        if (t.n == 0 && (b + u) % (int)gridDim.x == cta) zeros = true;
+    });
+    if (zeros) tile_zeros<D, W>(a);
+    const RunCut run(total, gridDim.x);
     if (total == 0 || cta >= run.ctas) {
         pdl_wait();  // the join that follows waits for this grid: the streaming kernel's end is part of it
         return;

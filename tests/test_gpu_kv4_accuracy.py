@@ -253,3 +253,38 @@ def test_scores_of_any_finite_magnitude(n, rows, d, q, scale):
         want = (values.cumsum(0) / torch.arange(1, n + 1, device="cuda")[:, None])[first:, None]
         assert abs(s) < 1e-10 and bars.relative(got, want) <= bars.relative_bar(torch.bfloat16)
     assert sx().device_error() == 0
+
+
+# ------------------------------------------------------------------ rows that see nothing
+@pytest.mark.parametrize("d,heads,kv_heads", [(64, 4, 2), (128, 32, 8), (256, 16, 1)])
+@pytest.mark.parametrize("lens,window", [([(0, 4000), (5000, 1)], 0), ([(10, 1700), (0, 513), (5000, 1), (0, 1)], 0),
+                                         ([(0, 3)] * 500 + [(300, 2), (100, 400)], 0), ([(0, 200), (7, 1)] * 60, 9)])
+def test_rows_without_keys_are_zero_and_others_count_every_key(d, heads, kv_heads, lens, window):
+    """Whole requests without keys, and blocks of rows before the first key."""
+    st = Counted(79 + d, d, torch.float16, heads, kv_heads, 16, lens, window)
+    out = torch.full_like(st.q, 7.0)
+    st.run(out=out)
+    st.check(out)
+    row = 0
+    for n, r in lens:
+        assert not out[row:row + max(0, r - n)].any()
+        if n and r > n:
+            want = bars.counts(n, n, d, st.blocks[lens.index((n, r))], window, "cuda")[:, None]
+            assert ((out[row + r - n:row + r].double() - want).abs() <= bars.count_bar(want, torch.float16)).all()
+        row += r
+
+
+@pytest.mark.parametrize("rows", [3, 900])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_windows_past_a_narrow_table_see_nothing(d, rows):
+    """Rows whose window lies past the table's pages are 0; the others see the window's part that has pages."""
+    n, window, held = 3000, 40, 2560
+    st = Counted(83 + d, d, torch.float16, 8, 2, 16, [(n, rows)], window)
+    st.table = st.table[:, :held // 16].contiguous()
+    out = torch.full_like(st.q, 7.0)
+    st.run(out=out)
+    pos = torch.arange(n - rows, n, device="cuda")
+    assert not out[pos - window + 1 >= held].any()
+    whole = pos < held
+    want = bars.counts_at(pos[whole], d, st.blocks[0], window)[:, None]
+    assert ((out[whole].double() - want).abs() <= bars.count_bar(want, torch.float16)).all()
