@@ -288,3 +288,15 @@ def test_windows_past_a_narrow_table_see_nothing(d, rows):
     whole = pos < held
     want = bars.counts_at(pos[whole], d, st.blocks[0], window)[:, None]
     assert ((out[whole].double() - want).abs() <= bars.count_bar(want, torch.float16)).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("pairs", [60, 64, 68, 92, 96, 100, 128])
+@pytest.mark.parametrize("widest", [0, 200])
+def test_both_sides_of_the_kernel_choice(pairs, widest, d):
+    """Requests of 60 to 128 pairs a key head, alone (16 columns a unit) or beside a chunk (8)."""
+    st = Counted(89 + d, d, torch.float16, 8, 2, 64, [(2000, pairs // 4), (1000 + widest, max(1, widest)), (3, 1)])
+    st.check(st.run())
+    got = Centred(97 + d, d, torch.bfloat16, 8, 2, 64, [(2000, pairs // 4), (1500, max(1, widest))])
+    out, (want, _) = got.run(), got.want()
+    assert bars.relative(out, want) <= bars.relative_bar(torch.bfloat16)

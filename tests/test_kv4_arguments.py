@@ -150,3 +150,18 @@ def test_scales(scale, want):
     from test_kv4_host import attention
 
     assert attention(kv4._lib.load(), tokens=0, scale=scale) == want
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("max_q", [1, 16, 4096])
+def test_the_stated_size_of_a_call_is_admitted(head_dim, max_q):
+    """requests * kv_heads * table_width * page_size / 2 just below 2^31, in a few shapes; eight times that is refused
+    where a request may have many rows."""
+    from test_kv4_host import attention, cache
+
+    L = kv4._lib.load()
+    for requests, width in ((16, (1 << 32) // (16 * 2 * 64) - 64), (4096, (1 << 32) // (4096 * 2 * 64) - 64)):
+        c = cache(head_dim=head_dim)
+        assert attention(L, c, tokens=0, requests=requests, width=width, stride=width, max_q=max_q) == "SX_OK"
+        if max_q == 4096:
+            assert attention(L, c, tokens=0, requests=requests, width=8 * width, stride=8 * width, max_q=max_q) == "SX_ERR_BAD_SHAPE"
