@@ -76,7 +76,7 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     const long long steps = (long long)table_width * cache->page_size / (kKvGranule * (256 / D)) + 1 + kStPad;
     if ((double)units * (double)steps > INT_MAX) return SX_ERR_BAD_SHAPE;
     const long long blocks = (long long)tokens * (heads / cache->kv_heads) / kv4_tile_rows(D) + requests;
-    const long long tiles = (long long)table_width * cache->page_size / kv4_tile_keys(D) + 1 + kTlPad;
+    const long long tiles = (long long)table_width * cache->page_size / kv4_tile_keys(D) + 1 + kv4_tile_pad(D);
     if (most > few && (double)blocks * (double)tiles * cache->kv_heads > INT_MAX)
         return SX_ERR_BAD_SHAPE;
     if (tokens == 0) return SX_OK;

@@ -96,7 +96,8 @@ struct RunCut {
 // blocks of a key head follow one another, so all but the first find its cache in L2).  A unit that has steps
 // begins with kStPad empty ones, which stand for the time a CTA needs to begin and merge it (3 to 4 us, a
 // step of its four warps 0.4 us): without them the CTAs of short requests finished last (64 requests of
-// 1024 to 16384 keys: from 83 to 110 us).
+// 1024 to 16384 keys: from 83 to 110 us).  Measured with 4 / 8 / 16, us: 64 requests of 1024 to 16384 keys, 8 key heads
+// of 64, 71 / 66 / 69, of 128, 118 / 111 / 114; 4 of 256 to 8192 keys, 72 / 69 / 67.
 constexpr int kStWarps = 4;
 constexpr int kStRows = 16;  // columns of a partial slot
 constexpr int kStPad = 8;
@@ -115,10 +116,12 @@ __device__ __forceinline__ int stream_most(int total, int grid) { return min(gri
 
 // Tile kernel: a step is a tile of kv4_tile_keys(D) keys of one unit = (request, key head, block of
 // kv4_tile_rows(D) (row, query head) pairs).
-// A unit that has tiles begins with kTlPad empty ones in the list, which stand for the time a CTA needs to
-// begin and end it (about 8 us, a tile 3.6): without them the CTAs of short units finished last (a mixed
-// step: 172 us where the others took 110 to 140).
-constexpr int kTlPad = 2;
+// A unit that has tiles begins with kv4_tile_pad(D) empty ones in the list, which stand for the time a CTA
+// needs to begin and end it (about 8 us, a tile of D = 128 3.6): without them the CTAs of short units finished last.
+// Measured with 2 / 3 / 6, us: 3 chunks of 400 to 777 rows beside 29 single tokens, window 2048, D = 64
+// 126 / 126 / 133, D = 128 187 / 176 / 177, D = 256 268 / 260 / 241; 8 chunks of 150 to 300 rows, D = 64 76 / 76 / 81, D = 256
+// 267 / 245 / 221.
+__host__ __device__ constexpr int kv4_tile_pad(int D) { return D == 256 ? 6 : 3; }
 __host__ __device__ constexpr int kv4_tile_rows(int D) { return D == 256 ? 128 : 256; }
 __host__ __device__ constexpr int kv4_tile_keys(int D) { return D == 256 ? 64 : 128; }
 
@@ -139,7 +142,8 @@ __device__ __forceinline__ TileUnit tile_unit(const Kv4AttnArgs& a, const Kv4Req
     return t;
 }
 
-__device__ __forceinline__ int tile_list(int tiles) { return tiles > 0 ? tiles + kTlPad : 0; }  // a unit's share of the list
+template <int D>
+__device__ __forceinline__ int tile_list(int tiles) { return tiles > 0 ? tiles + kv4_tile_pad(D) : 0; }  // a unit's share of the list
 
 // A request's blocks; 0 for the streaming kernel's requests.
 template <int D>
@@ -217,7 +221,7 @@ __device__ __forceinline__ int tile_list_total(const Kv4AttnArgs& a, int* red, i
         for (int u = u0; u < blocks; u += du) {
             const TileUnit t = tile_unit<D>(a, r, u);
             each(b, r, t, u);
-            n += tile_list(t.n);
+            n += tile_list<D>(t.n);
         }
         return n;
     };
@@ -240,12 +244,12 @@ __device__ __forceinline__ void tile_list_find(const Kv4AttnArgs& a, int* red, i
         const Kv4Request r = kv4_request(a, b);
         const int blocks = tile_blocks<D>(a, r);
         int n = 0;
-        for (int u = 0; u < blocks; u++) n += tile_list(tile_unit<D>(a, r, u).n);
+        for (int u = 0; u < blocks; u++) n += tile_list<D>(tile_unit<D>(a, r, u).n);
         return n * a.kv_heads;
     });
     const Kv4Request r = kv4_request(a, pick[0]);
     const int blocks = tile_blocks<D>(a, r);
-    auto unit = [&](int u) { return u < blocks ? tile_list(tile_unit<D>(a, r, u).n) : 0; };
+    auto unit = [&](int u) { return u < blocks ? tile_list<D>(tile_unit<D>(a, r, u).n) : 0; };
     int head = 0, before;
     for (int u0 = 0; u0 < blocks; u0 += W * 32) head += block_scan<W>(unit(u0 + threadIdx.x), red, before);
     const int h = (at - pick[1]) / head, first = pick[1] + h * head;

@@ -184,12 +184,12 @@ __global__ void __launch_bounds__(kJoinThreads, 2) kv4_join_tile_kernel(Kv4AttnA
     const Kv4Request r = kv4_request(a, pick[0]);
     const TileUnit t = tile_unit<D>(a, r, pick[2]);
     const int u0 = pick[3], h = pick[4];
-    const int first = run.owner(u0 + kTlPad);  // of the unit's tiles
-    if (at <= u0 + kTlPad || first != cut - 1 || row0 >= t.rows) {
+    const int first = run.owner(u0 + kv4_tile_pad(D));  // of the unit's tiles
+    if (at <= u0 + kv4_tile_pad(D) || first != cut - 1 || row0 >= t.rows) {
         pdl_wait();
         return;
     }
-    const int shares = run.owner(u0 + kTlPad + t.n - 1) - first + 1, rows = min(t.rows - row0, ROWS);
+    const int shares = run.owner(u0 + kv4_tile_pad(D) + t.n - 1) - first + 1, rows = min(t.rows - row0, ROWS);
     constexpr size_t STRIDE = (size_t)kv4_tile_rows(D) * (D + 2);
     // a CTA's slots: its first segment, its last; the unit is the first CTA's last, unless its run began in it
     const float* s1 = a.part + (size_t)(2 * first) * STRIDE;

@@ -365,16 +365,16 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(con
     cur.b = pick[0];
     tile_load<D>(a, cur);
     cur.u = pick[2], cur.h = pick[4];
-    cur.beg = min(0, pick[3] + kTlPad - start);
+    cur.beg = min(0, pick[3] + kv4_tile_pad(D) - start);
     cur.t = tile_unit<D>(a, cur.r, cur.u);
     if (tid == 0) {
         // the run's tiles, less the units' empty ones
         const int end = run.start(cta + 1);
         TileCursor c = cur;
         int n = 0;
-        for (int p = pick[3]; p < end; p += tile_list(c.t.n)) {
+        for (int p = pick[3]; p < end; p += tile_list<D>(c.t.n)) {
             if (p > pick[3]) tile_seek<D>(a, c, c.beg + c.t.n);
-            n += max(0, min(end, p + tile_list(c.t.n)) - max(start, p + kTlPad));
+            n += max(0, min(end, p + tile_list<D>(c.t.n)) - max(start, p + kv4_tile_pad(D)));
         }
         run_tiles = n;
     }
