@@ -37,16 +37,25 @@ def _current(gpu):
     return _HERE if torch._C._cuda_getDevice() == gpu else torch.cuda.device(gpu)
 
 
+def _int(v):
+    """v as the library's 32-bit integers hold it; refused past them (ctypes would cut it)."""
+    v = int(v)
+    if not -(1 << 31) <= v < 1 << 31:
+        raise Exl3Error(1)
+    return v
+
+
 class Kv4Cache:
     """A pool of pages for one layer's keys and values in 4 bits (sx_kv4): `pages` pages of
     `page_size` tokens (16, 32, 64, 128 or 256) of `kv_heads` heads of `head_dim` (64, 128 or 256)
     channels.  `pool`: an optional uint8 tensor to use, [pages, kv_heads, block_bytes]."""
 
     def __init__(self, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda", pool=None):
-        block = lib().sx_kv4_block_bytes(int(head_dim), int(page_size))
+        pages, kv_heads, head_dim, page_size = _int(pages), _int(kv_heads), _int(head_dim), _int(page_size)
+        block = lib().sx_kv4_block_bytes(head_dim, page_size)
         if block == 0 or pages < 1 or kv_heads < 1:
             raise Exl3Error(1)
-        self.pages, self.kv_heads, self.head_dim, self.page_size = int(pages), int(kv_heads), int(head_dim), int(page_size)
+        self.pages, self.kv_heads, self.head_dim, self.page_size = pages, kv_heads, head_dim, page_size
         if pool is None:
             pool = torch.empty((self.pages, self.kv_heads, block), dtype=torch.uint8, device=device)
         elif pool.dtype != torch.uint8:
@@ -100,7 +109,7 @@ def block_tables(ctx_lens, new_lens, table, free_pages, free_count, page_size: i
     c, n = _ints(ctx_lens, gpu), _ints(new_lens, gpu, requests)
     t, width, stride = _table(table, gpu, requests)
     f, fc = _ints(free_pages, gpu), _ints(free_count, gpu, 1)
-    tokens = int(tokens)
+    tokens, page_size = _int(tokens), _int(page_size)
     if tokens < 0:
         raise Exl3Error(1)
     with _current(gpu):
@@ -156,7 +165,7 @@ def kv4_read(cache: Kv4Cache, slots, dtype=torch.bfloat16):
 
 
 def kv4_attention_workspace_bytes(cache: Kv4Cache, requests: int, tokens: int, heads: int, max_q: int) -> int:
-    return lib().sx_kv4_attention_workspace_bytes(cache._ref, int(requests), int(tokens), int(heads), int(max_q))
+    return lib().sx_kv4_attention_workspace_bytes(cache._ref, _int(requests), _int(tokens), _int(heads), _int(max_q))
 
 
 class _Kept:
@@ -188,6 +197,7 @@ def kv4_attention(q, cache: Kv4Cache, table, kv_lens, cu_q, max_q: int, scale=No
     if q.dim() != 3:
         raise Exl3Error(1)
     tokens, heads, _ = q.shape
+    max_q, window = _int(max_q), _int(min(window, (1 << 31) - 1))  # a window wider than any cache is none
     gpu = cache.gpu
     qp, ts, hs = _rows(q, gpu, heads, cache.head_dim)
     requests = kv_lens.numel()

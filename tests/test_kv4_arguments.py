@@ -165,3 +165,16 @@ def test_the_stated_size_of_a_call_is_admitted(head_dim, max_q):
         assert attention(L, c, tokens=0, requests=requests, width=width, stride=width, max_q=max_q) == "SX_OK"
         if max_q == 4096:
             assert attention(L, c, tokens=0, requests=requests, width=8 * width, stride=8 * width, max_q=max_q) == "SX_ERR_BAD_SHAPE"
+
+
+def test_integers_past_32_bits_are_refused_or_none(rec, monkeypatch):
+    c, t = cache(rec, monkeypatch), tensors()
+    attend(c, t, window=(1 << 32) + 16)  # wider than any cache: no window, and not one of 16
+    assert rec.calls[-1][1][-4] == (1 << 31) - 1
+    past = (1 << 32) + 16
+    for call in (lambda: attend(c, t, max_q=past), lambda: attend(c, t, window=-past),
+                 lambda: kv4.block_tables(t["ctx"], t["new"], t["table"], t["free"], t["count"], past, 2),
+                 lambda: kv4.Kv4Cache(1, 1, 64, past), lambda: kv4.kv4_attention_workspace_bytes(c, 1, 1, 1, past)):
+        with pytest.raises(Exl3Error, match="SX_ERR_BAD_SHAPE"):
+            call()
+    assert len(rec.calls) == 1
