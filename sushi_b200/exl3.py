@@ -167,7 +167,8 @@ def linear(x, proj: Proj, dec: Decode, flags: int = 0, out=None):
     if out is None:
         y = torch.empty((x.shape[0], out_f), dtype=x.dtype, device=x.device)
     else:
-        if out.shape != (x.shape[0], out_f) or out.dtype != x.dtype or not out.is_contiguous():
+        if out.shape != (x.shape[0], out_f) or out.dtype != x.dtype or not out.is_contiguous() \
+                or out.get_device() != proj.trellis.get_device():  # the kernel follows its pointer
             raise Exl3Error(1)
         y = out
     p, d = proj.c(), dec.c()
