@@ -375,8 +375,8 @@ sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slot
  * positions 0 .. kv_lens[b], the step's own tokens last (written before this call).  Row i stands at
  * position p = kv_lens[b] - q_len + i and sees positions <= p, and > p - window when window > 0:
  *   out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j      (k, v of head h * kv_heads / heads)
- * with f32 sums; operands of the products (query, probability times step, or held key and value where
- * a request has many rows) are rounded to F16.  A row that sees nothing (kv_len 0, or q_len >
+ * with f32 sums.  BF16 calls round operands of the products to F16 (probability times step; probability, held key
+ * and held value where a request has many rows), F16 calls keep them in two F16 parts.  A row that sees nothing (kv_len 0, or q_len >
  * kv_len), and rows past cu_q[requests], are 0.
  * Positions whose page id is outside the pool, or past table_width pages, count as unseen.
  * q [tokens][heads][head_dim] with strides in elements, channels contiguous; out contiguous and

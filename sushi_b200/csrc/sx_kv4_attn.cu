@@ -27,8 +27,9 @@ namespace {
 //            2 x 32768         66 / 114     90 / 118    111 / 122    146 / 127
 //            16 x 8192        120 / 123    146 / 126    202 / 132    256 / 138
 //            64 x 1024         70 / 97      84 / 105    118 / 102    151 / 116
-// (F16: the streaming kernel 5 to 20% slower, the tile kernel the same.)  Many long requests would turn to the
-// tile kernel earlier, few requests later; the host does not know the lengths.
+// (F16: the streaming kernel 5 to 20% slower, the tile kernel, with its second parts, 5 to 50%; the same choice, a
+// little early: 64 / 96 pairs at D = 128, 16 x 8192 keys, 88 / 101 and 115 / 103.)  Many long requests would turn to
+// the tile kernel earlier, few requests later; the host does not know the lengths.
 constexpr int stream_pairs(int D) { return D == 64 ? 96 : 64; }
 
 // The widest request of a call, in pairs a key head.

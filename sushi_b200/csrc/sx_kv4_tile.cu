@@ -14,6 +14,12 @@
 // turns: one's softmax runs under the other's products.  The reference moves only when a score passes
 // it by 2^8 (P's best at 2^7, at most 2^15).
 //
+// Precision.  bf16 calls round held keys and values, and P, to F16 once (11 bits): outputs are 4.6e-4 off beyond
+// their own rounding of 1.66e-3 (1.72e-3 in all).  F16 outputs would show it (4.5e-4 to 5.7e-4 in all, of 2.1e-4 of their
+// own), so F16 calls (FINE) keep each in two F16 parts, with a second product for the scores and two more for the values:
+// 2.08e-4 in all, for 1.1 to 1.7 times the time (a 4096-row chunk over 8192 keys 1072 us, 648 in bf16).  Sums are f32, cut at each of the MMA's additions: over 131072 keys
+// of one unit outputs come 1.1e-4 short.
+//
 // Work: the units' tiles laid end to end and cut into equal runs, one a CTA (one CTA an SM), so
 // causal lengths balance and few long rows are split; a unit of several CTAs is joined by
 // sx_kv4_join.cu.  Every wait is bounded (sx_common.cuh).
@@ -29,13 +35,14 @@
 
 namespace sx {
 
-template <int D>
+template <int D, bool FINE>
 struct TileLayout {
     static constexpr int G = D / kKvGroup;
     static constexpr int MT = kv4_tile_rows(D) / 128;
     static constexpr int NK = kv4_tile_keys(D);
     static constexpr int NG = NK / kKvGranule;  // granules a tile
-    static constexpr int KST = 2, VST = D == 256 ? 1 : 2;
+    static constexpr int PARTS = FINE ? 2 : 1;  // of a key or value tile: leading, then trailing
+    static constexpr int KST = FINE && D >= 128 ? 1 : 2, VST = D == 256 || (FINE && D == 128) ? 1 : 2;
     // Widening warps.  7 beside 8 softmax warps and the MMA warp: 16, so 128 registers a thread.  Every
     // warp must have a task among a tile's keys (and among its values) in every tile or in none: a wait by
     // parity tells only neighbouring phases of a stage apart.
@@ -45,14 +52,14 @@ struct TileLayout {
     static constexpr int MMA_WARP = SM_WARPS + WIDEN;
     static constexpr int THREADS = (MMA_WARP + 1) * 32;
     static constexpr int HB = kv4_granule_bytes(D) / 2;  // a granule's keys, or its values
-    static constexpr int RING = D == 128 ? 3 : (D == 64 ? 6 : 2);
+    static constexpr int RING = D == 128 ? 3 : (D == 64 ? 6 : (FINE ? 1 : 2));
     static constexpr int Q_TILE = 128 * D * 2;
-    static constexpr int KV_TILE = NK * D * 2;
+    static constexpr int KV_TILE = NK * D * 2;  // one part
     static constexpr int SUB = NK * 128;  // bytes of 64 channels of a key tile
     static constexpr int Q = 0;
     static constexpr int K = Q + MT * Q_TILE;
-    static constexpr int V = K + KST * KV_TILE;
-    static constexpr int RAW = V + VST * KV_TILE;
+    static constexpr int V = K + KST * PARTS * KV_TILE;
+    static constexpr int RAW = V + VST * PARTS * KV_TILE;
     static constexpr int BAD = RAW + WIDEN * RING * HB;  // [VST][G][NG] u16: keys whose value group holds NaN
     static constexpr int GONE = BAD + VST * G * NG * 2;     // [4][NG] u8: granules without a page
     static constexpr int BAR = (GONE + 4 * NG + 15) / 16 * 16;
@@ -196,38 +203,65 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) 
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Eight codes as F16 pairs (0 4, 1 5, 2 6, 3 7), times s2 plus m2.  A code under 1024's exponent is
-// 1024 + code (or 1024 + 16 code), made the code itself exactly before the one rounding.
-__device__ __forceinline__ uint4 widen8(uint32_t x, __half2 s2, __half2 m2) {
+__device__ __forceinline__ uint32_t dup_lo(uint32_t p) { return __byte_perm(p, p, 0x1010); }
+__device__ __forceinline__ uint32_t dup_hi(uint32_t p) { return __byte_perm(p, p, 0x3232); }
+__device__ __forceinline__ __half2 as_half2(uint32_t p) { return *reinterpret_cast<const __half2*>(&p); }
+
+// Eight codes as F16 pairs (0 4, 1 5, 2 6, 3 7), times the step plus the minimum of each of PARTS parameters.
+// A code under 1024's exponent is 1024 + code (or 1024 + 16 code), made the code itself exactly before the one rounding.
+template <int PARTS>
+__device__ __forceinline__ void widen8(uint32_t x, const uint32_t (&par)[PARTS], uint4 (&out)[PARTS]) {
     const __half2 k1024 = __half2half2(__ushort_as_half((unsigned short)0x6400));
     const __half2 k16 = __half2half2(__ushort_as_half((unsigned short)0x2c00));  // 1/16
     const __half2 k64 = __half2half2(__ushort_as_half((unsigned short)0xd400));  // -64
     const uint32_t y = x >> 8;
     const uint32_t w[4] = {(x & 0x000f000fu) | 0x64006400u, (x & 0x00f000f0u) | 0x64006400u,
                            (y & 0x000f000fu) | 0x64006400u, (y & 0x00f000f0u) | 0x64006400u};
-    uint32_t o[4];
+    uint32_t o[PARTS][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
+        const __half2 h = as_half2(w[i]);
         const __half2 c = i & 1 ? __hfma2(h, k16, k64) : __hsub2(h, k1024);
-        const __half2 v = __hfma2(c, s2, m2);
-        o[i] = *reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+        for (int k = 0; k < PARTS; k++) {
+            const __half2 v = __hfma2(c, as_half2(dup_lo(par[k])), as_half2(dup_hi(par[k])));
+            o[k][i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
     }
-    return make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+    for (int k = 0; k < PARTS; k++) out[k] = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
 }
 
-__device__ __forceinline__ uint32_t dup_lo(uint32_t p) { return __byte_perm(p, p, 0x1010); }
-__device__ __forceinline__ uint32_t dup_hi(uint32_t p) { return __byte_perm(p, p, 0x3232); }
-__device__ __forceinline__ __half2 as_half2(uint32_t p) { return *reinterpret_cast<const __half2*>(&p); }
+// A step and minimum p as the sum of two: `lead` multiples of 2^-8 of the group's largest power of two, so that
+// code * s + m is exact in F16, `trail` what is left (code * s + m of it below 2^-4 of that power, rounded once).
+__device__ __forceinline__ void split_params(uint32_t p, uint32_t& lead, uint32_t& trail) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+    const float most = fmaxf(fabsf(f.y), fabsf(fmaf(15.0f, f.x, f.y)));
+    // 1.5 * 2^15 times that power: its last bit is 2^-8 of the power
+    const float grid = __uint_as_float(((__float_as_uint(most) & 0x7f800000u) + (15u << 23)) | 0x00400000u);
+    const float s = (f.x + grid) - grid, m = (f.y + grid) - grid;
+    const __half2 a = __floats2half2_rn(s, m), b = __floats2half2_rn(f.x - s, f.y - m);
+    lead = *reinterpret_cast<const uint32_t*>(&a);
+    trail = *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// A word's eight values to one 16-byte chunk, or their two parts to chunks TRAIL bytes apart.
+template <int PARTS, int TRAIL>
+__device__ __forceinline__ void widen_store(uint32_t x, const uint32_t (&par)[PARTS], uint8_t* out) {
+    uint4 v[PARTS];
+    widen8(x, par, v);
+#pragma unroll
+    for (int k = 0; k < PARTS; k++) *reinterpret_cast<uint4*>(out + k * TRAIL) = v[k];
+}
 
 // The channel of eight that sits at place p of a chunk.
 __host__ __device__ constexpr int chunk_channel(int p) { return (p >> 1) + 4 * (p & 1); }
 
 // The keys of a granule as rows row0 .. row0 + 15 of a tile; tokens from `live` on become 0.  Lanes: words
 // 2t and 2t + 1 of every group of one token, eight tokens at a time.
-template <int D>
+template <int D, bool FINE>
 __device__ __forceinline__ void widen_keys(const uint8_t* gran, int live, int row0, uint8_t* out) {
-    using L = TileLayout<D>;
+    using L = TileLayout<D, FINE>;
     constexpr int G = L::G;
     const int lane = threadIdx.x & 31, t = lane & 3;
     uint32_t x[2][G][2], p[2][G];
@@ -254,11 +288,11 @@ __device__ __forceinline__ void widen_keys(const uint8_t* gran, int live, int ro
     for (int hf = 0; hf < 2; hf++)
 #pragma unroll
         for (int gr = 0; gr < G; gr++) {
-            const __half2 s2 = as_half2(dup_lo(p[hf][gr])), m2 = as_half2(dup_hi(p[hf][gr]));
+            uint32_t par[L::PARTS] = {p[hf][gr]};
+            if constexpr (FINE) split_params(p[hf][gr], par[0], par[1]);
 #pragma unroll
             for (int i = 0; i < 2; i++)
-                *reinterpret_cast<uint4*>(out + gr * L::SUB + sw128_offset(row0 + hf * 8 + (lane >> 2), (2 * t + i) * 8)) =
-                    widen8(x[hf][gr][i], s2, m2);
+                widen_store<L::PARTS, L::KV_TILE>(x[hf][gr][i], par, out + gr * L::SUB + sw128_offset(row0 + hf * 8 + (lane >> 2), (2 * t + i) * 8));
         }
 }
 
@@ -266,9 +300,9 @@ __device__ __forceinline__ void widen_keys(const uint8_t* gran, int live, int ro
 // groups become 0 (a key some row does not see must not reach it) and are named in bad[group] for the rows
 // that do see them; the writer gives both parameters NaN or neither.  Lanes: word lane % 8 of every group of
 // one token, four tokens at a time.
-template <int D>
+template <int D, bool FINE>
 __device__ __forceinline__ void widen_values(const uint8_t* gran, int live, int row0, uint8_t* out, uint16_t* bad) {
-    using L = TileLayout<D>;
+    using L = TileLayout<D, FINE>;
     constexpr int G = L::G;
     const int lane = threadIdx.x & 31, pc = lane & 7;
     uint32_t x[4][G], p[4][G], nan[G];
@@ -311,14 +345,16 @@ __device__ __forceinline__ void widen_values(const uint8_t* gran, int live, int 
 #pragma unroll
     for (int q4 = 0; q4 < 4; q4++)
 #pragma unroll
-        for (int gr = 0; gr < G; gr++)
-            *reinterpret_cast<uint4*>(out + gr * L::SUB + sw128_offset(row0 + q4 * 4 + (lane >> 3), pc * 8)) =
-                widen8(x[q4][gr], as_half2(dup_lo(p[q4][gr])), as_half2(dup_hi(p[q4][gr])));
+        for (int gr = 0; gr < G; gr++) {
+            uint32_t par[L::PARTS] = {p[q4][gr]};
+            if constexpr (FINE) split_params(p[q4][gr], par[0], par[1]);
+            widen_store<L::PARTS, L::KV_TILE>(x[q4][gr], par, out + gr * L::SUB + sw128_offset(row0 + q4 * 4 + (lane >> 3), pc * 8));
+        }
 }
 
-template <int D>
-__global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(const __grid_constant__ Kv4AttnArgs a) {
-    using L = TileLayout<D>;
+template <int D, bool FINE>
+__global__ void __launch_bounds__(TileLayout<D, FINE>::THREADS, 1) kv4_tile_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    using L = TileLayout<D, FINE>;
     constexpr int G = L::G, MT = L::MT, NK = L::NK, NG = L::NG;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_slot;
@@ -576,15 +612,40 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(con
                     for (int i = 0; i < 16; i++) {
                         const float p0 = ex2(fmaf(__uint_as_float(v[2 * i]), c, -mref));
                         const float p1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), c, -mref));
+                        if constexpr (FINE) v[2 * i] = __float_as_uint(p0), v[2 * i + 1] = __float_as_uint(p1);
                         l4[i & 3] += p0 + p1;
                         const __half2 h = __floats2half2_rn(p0, p1);
                         w[i] = *reinterpret_cast<const uint32_t*>(&h);
                     }
                 };
+                // FINE: the weights of 32 columns go over them, in two parts of 16 columns
+                auto both = [&](uint32_t (&v)[32], uint32_t (&w)[32]) {
+                    weights(v, w);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                        const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * i]) - r.x, __uint_as_float(v[2 * i + 1]) - r.y);
+                        w[16 + i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                };
+#pragma unroll 1
+                for (int q = 0; FINE && q < NK; q += 64) {
+                    uint32_t w[32];
+                    tmem_ld32_wait(va);
+                    tmem_ld32_start(s_tm + q + 32, vb);
+                    both(va, w);
+                    __syncwarp();
+                    tmem_ld32_wait(vb);
+                    tmem_st32u(s_tm + q, w);
+                    if (q + 64 < NK) tmem_ld32_start(s_tm + q + 64, va);
+                    both(vb, w);
+                    __syncwarp();
+                    tmem_st32u(s_tm + q + 32, w);
+                }
                 // the weights of columns q go over columns q / 2, which are in registers by then; 64 at a
                 // time, since a store holds up the warp's later loads while the products run
 #pragma unroll 1
-                for (int q = 0; q < NK; q += 64) {
+                for (int q = 0; !FINE && q < NK; q += 64) {
                     uint32_t w[32];
                     tmem_ld32_wait(va);
                     tmem_ld32_start(s_tm + q + 32, vb);
@@ -716,13 +777,13 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(con
                 if (ok && tile >= L::KST) ok = mbar_wait(&kempty[stage], (tile / L::KST - 1) & 1, DEV_TIMEOUT_EMPTY);
                 if (ok) ok = mbar_wait(&bar[place], parity, DEV_TIMEOUT_FULL);
                 if (lane == 0) smem[L::GONE + (tile & 3) * NG + gi] = !got && first < cur.r.hi;
-                widen_keys<D>(raw, live, gi * kKvGranule, smem + L::K + stage * L::KV_TILE);
+                widen_keys<D, FINE>(raw, live, gi * kKvGranule, smem + L::K + stage * L::PARTS * L::KV_TILE);
             } else {
                 const int stage = (int)(tile % L::VST);
                 full = &vfull[stage];
                 if (ok && tile >= L::VST) ok = mbar_wait(&vempty[stage], (tile / L::VST - 1) & 1, DEV_TIMEOUT_EMPTY);
                 if (ok) ok = mbar_wait(&bar[place], parity, DEV_TIMEOUT_FULL);
-                widen_values<D>(raw - kv4_value_off(D), live, gi * kKvGranule, smem + L::V + stage * L::KV_TILE,
+                widen_values<D, FINE>(raw - kv4_value_off(D), live, gi * kKvGranule, smem + L::V + stage * L::PARTS * L::KV_TILE,
                                 reinterpret_cast<uint16_t*>(smem + L::BAD) + stage * (G * NG) + gi);
             }
             fence_proxy_async_smem();
@@ -739,22 +800,33 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(con
         uint32_t turn[2] = {0, 0};
         bool ok = true;
         auto scores = [&](int mt, int bi, uint32_t tile) {
-            const uint32_t q = smem_u32(smem + L::Q + mt * L::Q_TILE), k = smem_u32(smem + L::K + (tile % L::KST) * L::KV_TILE);
+            const uint32_t q = smem_u32(smem + L::Q + mt * L::Q_TILE), k = smem_u32(smem + L::K + (tile % L::KST) * L::PARTS * L::KV_TILE);
             if (ok) {
 #pragma unroll
-                for (int kk = 0; kk < D / 16; kk++)
-                    tc_mma_f16(tmem + L::S_COL + bi * NK, smem_desc_sw128(q + (kk >> 2) * 16384 + (kk & 3) * 32),
-                               smem_desc_sw128(k + (kk >> 2) * L::SUB + (kk & 3) * 32), id_s, kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < L::PARTS * (D / 16); kk++) {
+                    const int part = kk / (D / 16), k16 = kk % (D / 16);
+                    tc_mma_f16(tmem + L::S_COL + bi * NK, smem_desc_sw128(q + (k16 >> 2) * 16384 + (k16 & 3) * 32),
+                               smem_desc_sw128(k + part * L::KV_TILE + (k16 >> 2) * L::SUB + (k16 & 3) * 32), id_s, kk > 0 ? 1u : 0u);
+                }
             }
             tc_commit(&sfull[bi]);
         };
         auto values = [&](int mt, int bi, uint32_t tile, bool first) {
-            const uint32_t v = smem_u32(smem + L::V + (tile % L::VST) * L::KV_TILE);
+            const uint32_t v = smem_u32(smem + L::V + (tile % L::VST) * L::PARTS * L::KV_TILE);
+            const uint32_t o = tmem + L::O_COL + mt * D, p = tmem + L::S_COL + bi * NK;
             if (ok) {
 #pragma unroll
-                for (int kk = 0; kk < NK / 16; kk++)
-                    tc_mma_ts_f16(tmem + L::O_COL + mt * D, tmem + L::S_COL + bi * NK + kk * 8,
-                                  smem_desc_sw128_n(v + kk * 2048, L::SUB), id_o, (!first || kk > 0) ? 1u : 0u);
+                for (int kk = 0; kk < NK / 16; kk++) {
+                    const uint64_t lead = smem_desc_sw128_n(v + kk * 2048, L::SUB);
+                    if constexpr (FINE) {  // all but the two trailing parts' product
+                        const uint32_t at = p + (kk >> 1) * 32 + (kk & 1) * 8;
+                        tc_mma_ts_f16(o, at, lead, id_o, (!first || kk > 0) ? 1u : 0u);
+                        tc_mma_ts_f16(o, at, smem_desc_sw128_n(v + L::KV_TILE + kk * 2048, L::SUB), id_o, 1u);
+                        tc_mma_ts_f16(o, at + 16, lead, id_o, 1u);
+                    } else {
+                        tc_mma_ts_f16(o, p + kk * 8, lead, id_o, (!first || kk > 0) ? 1u : 0u);
+                    }
+                }
             }
             tc_commit(&odone[MT == 2 ? mt : 0]);
         };
@@ -811,10 +883,10 @@ __global__ void __launch_bounds__(TileLayout<D>::THREADS, 1) kv4_tile_kernel(con
 
 namespace {
 
-template <int D>
+template <int D, bool FINE>
 cudaError_t tile_launch(const Kv4AttnArgs& a, cudaStream_t stream) {
-    using L = TileLayout<D>;
-    auto kern = kv4_tile_kernel<D>;
+    using L = TileLayout<D, FINE>;
+    auto kern = kv4_tile_kernel<D, FINE>;
     cudaError_t e = func_attrs(reinterpret_cast<const void*>(kern), L::ALLOC, false);
     if (e != cudaSuccess) return e;
     // starts as the streaming kernel drains: neither reads what the other writes
@@ -834,9 +906,10 @@ cudaError_t tile_launch(const Kv4AttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t kv4_tile_launch(const Kv4AttnArgs& a, int D, cudaStream_t stream) {
-    if (D == 64) return tile_launch<64>(a, stream);
-    if (D == 128) return tile_launch<128>(a, stream);
-    return tile_launch<256>(a, stream);
+    const bool fine = a.dt == SX_DT_F16;
+    if (D == 64) return fine ? tile_launch<64, true>(a, stream) : tile_launch<64, false>(a, stream);
+    if (D == 128) return fine ? tile_launch<128, true>(a, stream) : tile_launch<128, false>(a, stream);
+    return fine ? tile_launch<256, true>(a, stream) : tile_launch<256, false>(a, stream);
 }
 
 }  // namespace sx

@@ -20,7 +20,9 @@ beyond rounding: what an output is off by that its own rounding does not explain
     sqrt(error^2 - rounding^2) of their norms against the outputs'.  A probability times step of 11 bits is off
     by 2.1e-4 (rms); where that counts against the value's own size it gives 2.1e-4 here.  64 normal channels span
     about 4.8 deviations, 15 steps: against the whole code (0 to 15) it would be 2.6 times as much, 5.5e-4.
-    The bar is 3.2e-4, one and a half of the former."""
+    The bar is 3.2e-4, one and a half of the former.  F16 outputs, where operands are kept in two parts of 11
+    bits, 2^-18 and less: what is left are f32 sums that the matrix unit cuts, 1e-4 at a few thousand keys; that
+    is half their own rounding, and below any one operand of 11 bits."""
 
 import torch
 
@@ -64,7 +66,7 @@ def count_bar(want, dtype):
     return want * (UNIT[dtype] + 2.0 ** -20)
 
 
-BEYOND_BAR = 3.2e-4
+BEYOND_BAR = {torch.bfloat16: 3.2e-4, torch.float16: 1e-4}
 
 
 def beyond_rounding(got, want):

@@ -72,7 +72,7 @@ def test_sums_do_not_drift_over_long_caches(n, requests, rows, heads, kv_heads, 
 @pytest.mark.parametrize("rows,heads,kv_heads,d", [(2, 32, 8, 128), (16, 32, 8, 128), (4, 32, 8, 64), (2, 16, 4, 256), (4, 64, 8, 256)])
 def test_bf16_outputs_of_few_rows_are_off_by_little_more_than_their_rounding(rows, heads, kv_heads, d):
     st = Shared(rows + d, 6000, 2, rows, heads, kv_heads, d, torch.bfloat16)
-    assert bars.beyond_rounding(st.run(), st.want()[None].expand(2, -1, -1, -1)) <= bars.BEYOND_BAR
+    assert bars.beyond_rounding(st.run(), st.want()[None].expand(2, -1, -1, -1)) <= bars.BEYOND_BAR[torch.bfloat16]
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
@@ -300,3 +300,27 @@ def test_both_sides_of_the_kernel_choice(pairs, widest, d):
     got = Centred(97 + d, d, torch.bfloat16, 8, 2, 64, [(2000, pairs // 4), (1500, max(1, widest))])
     out, (want, _) = got.run(), got.want()
     assert bars.relative(out, want) <= bars.relative_bar(torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,d", [(2, 32, 8, 128), (4, 32, 8, 64), (2, 16, 4, 256), (40, 32, 8, 128), (300, 4, 1, 128),
+                                                   (130, 16, 8, 64), (70, 8, 4, 256), (9, 32, 2, 256)])
+@pytest.mark.parametrize("n", [700, 6000])
+def test_f16_outputs_are_off_by_little_more_than_their_rounding(rows, heads, kv_heads, d, n):
+    st = Shared(rows + d, n, 2, rows, heads, kv_heads, d, torch.float16)
+    assert bars.beyond_rounding(st.run(), st.want()[None].expand(2, -1, -1, -1)) <= bars.BEYOND_BAR[torch.float16]
+
+
+@pytest.mark.parametrize("rows", [1, 120])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("gain,shift", [(1e-4, 0.0), (1.0, 30.0), (500.0, -2e4), (3e3, 1e4)])
+def test_f16_values_of_any_magnitude_keep_their_bits(gain, shift, d, rows):
+    """Values around 1e-4 to those near the format's largest, with and without a mean: the error of a row
+    against its values' size, which is what the parts of a value are taken against."""
+    st = Shared(rows + d, 3000, 2, rows, 4, 2, d, torch.float16)
+    st.v = (st.v.float() * gain + shift).half()
+    pages = st.table.shape[1]
+    pos = torch.arange(st.n, device="cuda")
+    sx().kv4_write(st.cache, st.k, st.v, st.table[0].long()[pos // 64] * 64 + pos % 64)
+    want, size = st.want()[None], ref.held(st.v)[0].abs().max()
+    err = (st.run().double() - want).abs()
+    assert pages and (err <= 2.0 ** -11 * want.abs() + 2.0 ** -15 * size + 2.0 ** -25).all()
