@@ -62,8 +62,10 @@ def counts(n, rows, d, block, window=0, device="cpu"):
 
 
 def count_bar(want, dtype):
-    """The allowed error of each output (a channel without visible keys is 0 exactly)."""
-    return want * (UNIT[dtype] + 2.0 ** -20)
+    """The allowed error of each output (a channel without visible keys is 0 exactly): half the type's spacing, which
+    for F16 does not shrink below 2^-24, and 2^-20 of it."""
+    half = (want * UNIT[dtype]).clamp(min=2.0 ** -25 if dtype == torch.float16 else 0.0)
+    return torch.where(want > 0, half + want * 2.0 ** -20, torch.zeros_like(want))
 
 
 BEYOND_BAR = {torch.bfloat16: 3.2e-4, torch.float16: 1e-4}

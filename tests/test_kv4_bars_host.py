@@ -67,3 +67,12 @@ def test_the_counts_are_the_definition(window):
         pos = n - rows + i
         seen = v[max(0, pos - window + 1) if window else 0:pos + 1].double()
         assert torch.allclose(seen.mean(0), want, rtol=1e-14, atol=0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,rows,d", [(700, 700, 64), (20000, 9000, 128), (131071, 50, 256)])
+def test_rounded_counts_are_within_the_bar(n, rows, d, dtype):
+    """F16 outputs below 2^-14 round to multiples of 2^-24."""
+    block = -(-n // d)
+    want = bars.counts(n, rows, d, block)
+    assert ((want.to(dtype).double() - want).abs() <= bars.count_bar(want, dtype)).all()
