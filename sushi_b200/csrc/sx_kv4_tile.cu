@@ -17,8 +17,10 @@
 // Precision.  bf16 calls round held keys and values, and P, to F16 once (11 bits): outputs are 4.6e-4 off beyond
 // their own rounding of 1.66e-3 (1.72e-3 in all).  F16 outputs would show it (4.5e-4 to 5.7e-4 in all, of 2.1e-4 of their
 // own), so F16 calls (FINE) keep each in two F16 parts, with a second product for the scores and two more for the values:
-// 2.08e-4 in all, for 1.1 to 1.7 times the time (a 4096-row chunk over 8192 keys 1072 us, 648 in bf16).  Sums are f32, cut at each of the MMA's additions: over 131072 keys
-// of one unit outputs come 1.1e-4 short.
+// 2.08e-4 in all, for 1.1 to 1.7 times the time (a 4096-row chunk over 8192 keys 1072 us, 648 in bf16).  Sums are f32, cut (not rounded) at
+// each of the MMA's additions, so outputs come short with the tiles summed, in bf16 calls by 1.1e-4 over 131072 keys of
+// a CTA.  F16 calls, with three additions for one, sum at most MOST tiles in tensor memory and add them up in the
+// CTA's partial slot.
 //
 // Work: the units' tiles laid end to end and cut into equal runs, one a CTA (one CTA an SM), so
 // causal lengths balance and few long rows are split; a unit of several CTAs is joined by
@@ -66,6 +68,7 @@ struct TileLayout {
     static constexpr int NBAR = WIDEN * RING + 2 * KST + 2 * VST + 2 + 2 + 2 + 1;
     static constexpr int TOTAL = BAR + NBAR * 8;
     static constexpr int ALLOC = TOTAL + 1024;
+    static constexpr int MOST = FINE ? 64 : 1 << 30;  // tiles summed in tensor memory at a time
     static constexpr int S_COL = 0;  // two S tiles of NK columns
     static constexpr int O_COL = 256;
     static_assert(ALLOC <= 227 * 1024, "fits a CTA");
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(TileLayout<D, FINE>::THREADS, 1) kv4_tile_kern
             tile_seek<D>(a, cur, pos);
             const Kv4Request r = cur.r;
             const TileUnit un = cur.t;
-            const int seg_end = min(len, cur.beg + un.n);
+            const int unit_end = min(len, cur.beg + un.n), seg_end = min(unit_end, pos + min(L::MOST, len));
             const int j0 = pos - cur.beg, n = seg_end - pos;
             const int e = mt * 128 + row;
             const bool live = e < un.rows;              // this thread has a pair
@@ -681,12 +684,25 @@ __global__ void __launch_bounds__(TileLayout<D, FINE>::THREADS, 1) kv4_tile_kern
             tiles += n;
 
             // ---------------- the rows out, or this CTA's share of them into its slot
-            const bool whole = j0 == 0 && n == un.n;
-            float* slot = a.part + (size_t)(2 * cta + (pos == 0 ? 0 : 1)) * (kv4_tile_rows(D) * (D + 2));
+            const int begun = max(cur.beg, 0);  // the unit's first tile here
+            const bool whole = begun == cur.beg && seg_end == cur.beg + un.n;
+            float* slot = a.part + (size_t)(2 * cta + (begun == 0 ? 0 : 1)) * (kv4_tile_rows(D) * (D + 2));
             if (tile_live) {
                 if (ok) ok = mbar_wait(&odone[MT == 2 ? mt : 0], (turns - 1) & 1, DEV_TIMEOUT_FULL);
                 tc_fence_after();
-                const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+                float* ml = slot + kv4_tile_rows(D) * D + 2 * e;
+                float m = mref * (c_first / c), now = 1.0f;
+                [[maybe_unused]] float before = 0.0f;  // the weight of what this unit's tiles left in the slot before
+                const bool more = FINE && pos > begun;
+                if (more && live) {
+                    const float2 held = __ldcg(reinterpret_cast<const float2*>(ml));
+                    const float up = fmaxf(held.x, m);
+                    before = ex2(held.x - up), now = ex2(m - up);
+                    l = fmaf(l, now, held.y * before);
+                    m = up;
+                }
+                const float inv = whole ? (l == 0.0f ? 0.0f : now / l) : now;
+                if (whole) before = l == 0.0f ? 0.0f : before / l;
 #pragma unroll 1
                 for (int q = 0; q < D; q += 32) {
                     float v[32];
@@ -701,23 +717,29 @@ __global__ void __launch_bounds__(TileLayout<D, FINE>::THREADS, 1) kv4_tile_kern
                             float x[8];
 #pragma unroll
                             for (int i = 0; i < 8; i++) x[chunk_channel(i)] = v[w + i];
+                            float4* at = reinterpret_cast<float4*>(slot + e * D + q + w);
+                            if (more) {
+                                const float4 y = __ldcg(at), z = __ldcg(at + 1);
+                                x[0] = fmaf(before, y.x, x[0]), x[1] = fmaf(before, y.y, x[1]);
+                                x[2] = fmaf(before, y.z, x[2]), x[3] = fmaf(before, y.w, x[3]);
+                                x[4] = fmaf(before, z.x, x[4]), x[5] = fmaf(before, z.y, x[5]);
+                                x[6] = fmaf(before, z.z, x[6]), x[7] = fmaf(before, z.w, x[7]);
+                            }
                             if (whole) {
                                 *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (r.q0 + qi) * head_row +
                                                           (size_t)head * D + q + w) =
                                     make_uint4(pack_act2(x[0], x[1], a.dt), pack_act2(x[2], x[3], a.dt),
                                                pack_act2(x[4], x[5], a.dt), pack_act2(x[6], x[7], a.dt));
                             } else {
-                                float4* dst = reinterpret_cast<float4*>(slot + e * D + q + w);
-                                __stcg(dst, make_float4(x[0], x[1], x[2], x[3]));
-                                __stcg(dst + 1, make_float4(x[4], x[5], x[6], x[7]));
+                                __stcg(at, make_float4(x[0], x[1], x[2], x[3]));
+                                __stcg(at + 1, make_float4(x[4], x[5], x[6], x[7]));
                             }
                         }
                     }
                 }
                 __syncwarp();
                 tc_fence_before();  // the next unit's first product overwrites O after the next arrival
-                if (!whole && live)
-                    __stcg(reinterpret_cast<float2*>(slot + kv4_tile_rows(D) * D + 2 * e), make_float2(mref * (c_first / c), l));
+                if (!whole && live) __stcg(reinterpret_cast<float2*>(ml), make_float2(m, l));
             }
             pos = seg_end;
         }
@@ -832,7 +854,7 @@ __global__ void __launch_bounds__(TileLayout<D, FINE>::THREADS, 1) kv4_tile_kern
         };
         for (int pos = 0; pos < len;) {
             tile_seek<D>(a, cur, pos);
-            const int seg_end = min(len, cur.beg + cur.t.n);
+            const int seg_end = min(min(len, cur.beg + cur.t.n), pos + min(L::MOST, len));
             const int n = seg_end - pos;
             const int live = MT == 2 && cur.t.rows > 128 ? 2 : 1;
             if (ok) ok = mbar_wait(qfull, segs & 1, DEV_TIMEOUT_FULL);

@@ -324,3 +324,35 @@ def test_f16_values_of_any_magnitude_keep_their_bits(gain, shift, d, rows):
     want, size = st.want()[None], ref.held(st.v)[0].abs().max()
     err = (st.run().double() - want).abs()
     assert pages and (err <= 2.0 ** -11 * want.abs() + 2.0 ** -15 * size + 2.0 ** -25).all()
+
+
+# ------------------------------------------------------------------ units of many tiles
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens,window", [([(40000, 70)] * 4, 0), ([(9000, 70), (8257, 66)] * 12, 0), ([(20000, 9000)], 0), ([(30000, 1500)], 9500)])
+def test_units_of_many_tiles_count_every_key_once(lens, window, d, dtype):
+    """More tiles than an F16 call sums at a time in tensor memory, of whole units and of shared ones."""
+    n = max(n for n, _ in lens)
+    st = Counted(101 + d, d, dtype, 8, 4, 64, lens, window)
+    got = st.run()
+    if n // d < 240:  # one key shows beside the output's rounding
+        st.check(got)
+    assert torch.equal(got, st.run())
+    st = Centred(103 + d, d, dtype, 4, 2, 64, lens[:2], window)
+    got, row = st.run(), 0
+    for (n, r), k, v in zip(st.lens, st.k.split([n for n, _ in st.lens]), st.v.split([n for n, _ in st.lens])):
+        rows = torch.arange(0, r, max(1, r // 50), device="cuda")
+        kk, vv = ref.held(k)[0], ref.held(v)[0]
+        pos, key = n - r + rows[:, None], torch.arange(n, device="cuda")[None]
+        seen = (key <= pos) & (key > pos - window if window else key >= 0)
+        for h in range(4):
+            s = (st.q[row + rows, h].double() @ kk[:, h // 2].T * d ** -0.5).masked_fill(~seen, float("-inf"))
+            assert bars.relative(got[row + rows, h], torch.softmax(s, -1) @ vv[:, h // 2]) <= bars.relative_bar(dtype)
+        row += r
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,d", [(40, 16, 4, 128), (100, 4, 4, 64), (70, 4, 4, 256)])
+def test_f16_outputs_of_many_rows_over_long_caches(rows, heads, kv_heads, d):
+    """Units of hundreds of tiles a CTA: what the matrix unit cuts of its sums must not grow with them."""
+    st = Shared(107 + d, 60000, 40, rows, heads, kv_heads, d, torch.float16)
+    assert bars.beyond_rounding(st.run(), st.want()[None].expand(40, -1, -1, -1)) <= bars.BEYOND_BAR[torch.float16]
