@@ -12,17 +12,18 @@
 // up to three times the value it stands for, since code * s and m nearly cancel; so the minima's sum takes
 // P (m + 7.5 s) - 7.5 h, and what h lost counts against code - 7.5, which is of the value's size: 1.68e-3 off where
 // the bf16 output's own rounding is 1.67e-3 (1.74e-3 without; 114 -> 117 us for 64 requests).  F16 calls keep P * s
-// in two F16 parts with a second product (FINE; 2.2e-4 off of 2.1e-4).  m, sums and accumulators are f32.
+// in two F16 parts with a second product (FINE; 2.09e-4 off of 2.08e-4).  m, sums and accumulators are f32.
+//
+// The MMA's f32 sums, and the products within one, are cut, not rounded.  Codes are 0 to 15, so over a long cache
+// the codes' part and the minima's are hundreds of times their sum, the output, and what is cut of the one always has
+// its sign: at 131072 keys a CTA outputs were 5% off.  So every second granule is turned over: 15 - code (the
+// complement of the word, which costs nothing beside the masks) times -P * s, and P (m + 15 s) among the minima (bf16:
+// the 7.5 of above already does that).  The sums then stay near 0 and the cuts cancel; and every 16 steps the minima's
+// part moves into them, so that what is left does not depend on the length (131072 keys a CTA, relative: bf16 1.64e-3,
+// of which the output's own rounding is 1.63e-3; F16 2.2e-4 of 2.1e-4).
 //
 // The softmax reference of a column is kept so that P * s <= 2^15, whatever the values' magnitude:
 // it moves (one vote a step) only when a score or a step would pass that, with 2^4 to spare.
-//
-// The MMA's f32 sums are cut, not rounded, at each of their additions.  Over a long cache the codes' part
-// (codes are 0 to 15) and the minima's are hundreds of times their sum, the output, and a cut of 2^-24 of the
-// one at each granule grows with the length: at 131072 keys a CTA outputs were 5% off.  So every MOVE steps the
-// minima's part moves into the codes' sums, which are then of the output's size; the error no longer depends on
-// the length (131072 keys a CTA, relative: bf16 1.7e-3, of which the output's own rounding is 1.6e-3; F16
-// 2.7e-4 of 2.1e-4, 3.3e-4 with MOVE = 8).  64 requests of 1024 to 16384 keys: 110 us without, 114 with it.
 //
 // Work: the units' steps (4.5 KB of one head: 256/D granules of 16 tokens) laid end to end and cut
 // into equal runs, one a CTA, so ragged lengths balance; a CTA's warps take its steps in turn, each
@@ -128,7 +129,7 @@ template <int D, int NT, bool FINE>
 __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stream_kernel(Kv4AttnArgs a) {
     using L = StreamLayout<D, NT>;
     constexpr int G = L::G, GS = L::GS, COLS = L::COLS;
-    constexpr int MOVE = FINE ? 4 : 8;  // steps; an F16 output shows an error an eighth of bf16's
+    constexpr int MOVE = 16;  // steps between two moves of the minima's part
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int red[kStWarps], pick[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -340,6 +341,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
         const int full_lo = a.window > 0 ? r.pos0 + r.qn - a.window : 0;
         auto step = [&](const uint8_t* st, int p0, uint32_t vm, auto whole_step) {
             constexpr bool FULL = decltype(whole_step)::value;
+            const bool odd_step = mine / kStWarps & 1;
             // scores
             float x[GS][NT][4];
 #pragma unroll
@@ -468,7 +470,9 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
 #pragma unroll
             for (int gi = 0; gi < GS; gi++) {
                 const uint8_t* gran = st + gi * L::GB;
-                uint32_t pb[G][NT][2];                  // P * s
+                const bool turned = GS == 1 ? odd_step : gi & 1;
+                const uint32_t over = turned ? 0xffffffffu : 0u;
+                uint32_t pb[G][NT][2];                  // P * s, or -P * s
                 [[maybe_unused]] uint32_t pl[G][NT][2];  // FINE: what its rounding left
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -482,8 +486,9 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
 #pragma unroll
                         for (int rr = 0; rr < 2; rr++) {
                             const float2 vp = vpar[gi][rr][gr];
-                            float a0 = p[2 * rr] * vp.x, a1 = p[2 * rr + 1] * vp.x;
-                            const float mid = FINE ? vp.y : fmaf(7.5f, vp.x, vp.y);
+                            const float by = turned ? -vp.x : vp.x;
+                            float a0 = p[2 * rr] * by, a1 = p[2 * rr + 1] * by;
+                            const float mid = FINE ? (turned ? fmaf(15.0f, vp.x, vp.y) : vp.y) : fmaf(7.5f, vp.x, vp.y);
                             float b0 = p[2 * rr], b1 = p[2 * rr + 1], m0 = mid, m1 = mid;
                             if constexpr (!FULL) {  // a key one row sees and another does not may hold NaN
                                 if (x[gi][nt][2 * rr] == -CUDART_INF_F) a0 = m0 = 0.0f;
@@ -523,7 +528,7 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
                     const uint32_t w23[2] = {__byte_perm(vw[2][gr], vw[3][gr], 0x5410), __byte_perm(vw[2][gr], vw[3][gr], 0x7632)};
 #pragma unroll
                     for (int mt = 0; mt < 4; mt++) {
-                        const uint32_t xx = w01[mt >> 1] >> (8 * (mt & 1)), yy = w23[mt >> 1] >> (8 * (mt & 1));
+                        const uint32_t xx = (w01[mt >> 1] >> (8 * (mt & 1))) ^ over, yy = (w23[mt >> 1] >> (8 * (mt & 1))) ^ over;
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             mma16816(o[gr][mt][nt], xx & 0x000f000fu, xx & 0x00f000f0u, yy & 0x000f000fu, yy & 0x00f000f0u,

@@ -21,8 +21,9 @@ beyond rounding: what an output is off by that its own rounding does not explain
     by 2.1e-4 (rms); where that counts against the value's own size it gives 2.1e-4 here.  64 normal channels span
     about 4.8 deviations, 15 steps: against the whole code (0 to 15) it would be 2.6 times as much, 5.5e-4.
     The bar is 3.2e-4, one and a half of the former.  F16 outputs, where operands are kept in two parts of 11
-    bits, 2^-18 and less: what is left are f32 sums that the matrix unit cuts, 1e-4 at a few thousand keys; that
-    is half their own rounding, and below any one operand of 11 bits."""
+    bits, 2^-18 and less: what is left are f32 sums that the matrix unit cuts, each by 2^-24 of a sum that is
+    tens to hundreds of times the output; the bar is 1e-4, half the output's own rounding, and below any one
+    operand of 11 bits."""
 
 import torch
 

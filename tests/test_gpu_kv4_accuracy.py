@@ -356,3 +356,16 @@ def test_f16_outputs_of_many_rows_over_long_caches(rows, heads, kv_heads, d):
     """Units of hundreds of tiles a CTA: what the matrix unit cuts of its sums must not grow with them."""
     st = Shared(107 + d, 60000, 40, rows, heads, kv_heads, d, torch.float16)
     assert bars.beyond_rounding(st.run(), st.want()[None].expand(40, -1, -1, -1)) <= bars.BEYOND_BAR[torch.float16]
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,d", [(1, 32, 8, 128), (2, 32, 4, 64), (1, 16, 4, 256), (40, 16, 4, 128), (3, 64, 4, 128)])
+@pytest.mark.parametrize("n,requests", [(20000, 1), (131071, 1), (60000, 40)])
+def test_f16_outputs_of_long_caches_with_strong_channels(n, requests, rows, heads, kv_heads, d):
+    """Keys with a few channels four times the others: the weights of a granule's keys differ widely."""
+    st = Shared(n + d, n, requests, rows, heads, kv_heads, d, torch.float16)
+    g = gen(5)
+    st.k = (st.k.float() * (1.0 + 3.0 * (torch.rand((kv_heads, d), generator=g, device="cuda") < 0.05))).half()
+    pos = torch.arange(n, device="cuda")
+    sx().kv4_write(st.cache, st.k, st.v, st.table[0].long()[pos // 64] * 64 + pos % 64)
+    want = st.want()[None].expand(requests, -1, -1, -1)
+    assert bars.beyond_rounding(st.run(), want) <= bars.BEYOND_BAR[torch.float16] * (1 if n < 1e5 or rows < 40 else 2)
