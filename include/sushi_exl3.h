@@ -371,7 +371,7 @@ sx_status sx_kv4_read(sx_stream stream, const sx_kv4* cache, const int64_t* slot
 
 /* Attention over the cache, for single tokens, drafted tokens and prompt chunks, mixed in one call.
  * Request b's rows are q rows cu_q[b] .. cu_q[b+1] (q_len of them, at most max_q, which picks the
- * kernels: a longer request's rows may be left unwritten); its keys are
+ * kernels: a longer request's rows may come out NaN); its keys are
  * positions 0 .. kv_lens[b], the step's own tokens last (written before this call).  Row i stands at
  * position p = kv_lens[b] - q_len + i and sees positions <= p, and > p - window when window > 0:
  *   out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j      (k, v of head h * kv_heads / heads)

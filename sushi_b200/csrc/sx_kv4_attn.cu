@@ -98,12 +98,13 @@ sx_status sx_kv4_attention(sx_stream stream, const sx_kv4* cache, const void* q,
     a.scale_log2 = (float)(scale * 1.4426950408889634);
     a.window = window > (1 << 30) ? 0 : window;  // wider than any cache: none (and positions less it stay in 32 bits)
     a.max_cols = few;
+    a.alone = most <= few;
     a.cols = cols;
     a.part = static_cast<float*>(workspace);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e = kv4_stream_launch(a, D, s);
     if (e != cudaSuccess) return cuda_status(e, "kv4_attention stream launch");
-    if (most <= few)
+    if (a.alone)
         return cuda_status(kv4_join_launch(a, nullptr, D, s), "kv4_attention join launch");
     Kv4AttnArgs t = a;
     t.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + stream_bytes(D, a.cols));

@@ -22,6 +22,7 @@ struct Kv4AttnArgs {
     float scale_log2;  // scale * log2(e)
     int window;
     int max_cols;      // requests of at most this many (row, head) pairs a key head are the streaming kernel's
+    int alone;         // the tile kernel does not run: no request is said to be wider
     int cols;          // the pairs its units take: 8 or 16
     float* part;       // the kernel's partial slots, two a CTA (units that several CTAs share)
 };

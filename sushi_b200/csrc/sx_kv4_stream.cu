@@ -144,22 +144,25 @@ __global__ void __launch_bounds__(kStThreads, stream_resident<D, NT>()) kv4_stre
     pdl_release();
     const int cta = blockIdx.x;
     const int past = min(max(a.cu_q[a.requests], 0), a.tokens);  // rows from here on belong to no request
-    // no key to see: no unit writes the rows of such a request, CTA b % grid does
-    auto keyless = [&](const Kv4Request& r) { return r.qn > 0 && r.hi <= r.lo && r.qn * (long long)a.group <= a.max_cols; };
+    // no unit writes the rows of a request without a key to see (0), nor of one past the call's max_q that only the
+    // tile kernel could take (NaN): CTA b % grid does
+    auto wide = [&](const Kv4Request& r) { return r.qn * (long long)a.group > a.max_cols; };
+    auto keyless = [&](const Kv4Request& r) { return r.qn > 0 && r.hi <= r.lo && !wide(r); };
     bool zeros = false;
     auto steps = [&](int b) {
         const Kv4Request r = kv4_request(a, b);
         const int n = stream_steps<D>(a, r);
-        if (keyless(r) && b % (int)gridDim.x == cta) zeros = true;
+        if ((keyless(r) || (a.alone && wide(r))) && b % (int)gridDim.x == cta) zeros = true;
         return n > 0 ? stream_list(n) * a.kv_heads * stream_blocks(a, r) : 0;
     };
     int n0;
     const int total = list_total<kStWarps>(a.requests, red, n0, zeros, steps);
     for (int b = cta; zeros && b < a.requests; b += gridDim.x) {
         const Kv4Request r = kv4_request(a, b);
-        if (!keyless(r)) continue;
+        if (!keyless(r) && !(a.alone && wide(r))) continue;
+        const uint32_t fill = wide(r) ? 0x7fff7fffu : 0u;  // NaN in both types
         uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t)r.q0 * a.heads * D);
-        for (size_t i = tid; i < (size_t)r.qn * a.heads * D / 8; i += kStThreads) o[i] = make_uint4(0, 0, 0, 0);
+        for (size_t i = tid; i < (size_t)r.qn * a.heads * D / 8; i += kStThreads) o[i] = make_uint4(fill, fill, fill, fill);
     }
     const RunCut run(total, stream_most(total, gridDim.x));
     if (past < a.tokens) {

@@ -369,3 +369,22 @@ def test_f16_outputs_of_long_caches_with_strong_channels(n, requests, rows, head
     sx().kv4_write(st.cache, st.k, st.v, st.table[0].long()[pos // 64] * 64 + pos % 64)
     want = st.want()[None].expand(requests, -1, -1, -1)
     assert bars.beyond_rounding(st.run(), want) <= bars.BEYOND_BAR[torch.float16] * (1 if n < 1e5 or rows < 40 else 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_request_past_max_q_is_right_or_nan(d, dtype):
+    """A caller that understates max_q gets no stale memory: rows of a request that only the tile kernel could take
+    are NaN, the others right."""
+    lens = [(900, 1), (700, 100), (0, 90), (500, 3), (64, 1)]
+    st = Counted(109 + d, d, dtype, 8, 2, 16, lens)
+    right, out = st.run(), torch.full_like(st.q, 7.0)
+    st.max_q = 3
+    st.run(out=out)
+    wide = torch.zeros(st.rows, dtype=torch.bool, device="cuda")
+    wide[1:191] = True
+    assert torch.isnan(out[wide]).all()
+    st.blocks = [b for (_, r), b in zip(lens, st.blocks) if r < 90]
+    st.lens = [(n, r) for n, r in lens if r < 90]
+    st.check(out[~wide])
+    st.check(right[~wide])
