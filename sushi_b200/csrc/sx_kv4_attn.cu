@@ -52,7 +52,7 @@ extern "C" {
 
 size_t sx_kv4_attention_workspace_bytes(const sx_kv4* cache, int32_t requests, int32_t tokens, int32_t heads,
                                         int32_t max_q) {
-    (void)requests, (void)tokens;
+    (void)requests, (void)tokens;  // partial slots are the CTAs', two each, whatever the requests
     if (!cache || !kv4_dim_ok(cache->head_dim) || cache->kv_heads < 1 || heads < cache->kv_heads || max_q < 1) return 0;
     const int D = cache->head_dim, cols = stream_cols(cache, heads, max_q);
     return stream_bytes(D, cols) + (most_pairs(cache, heads, max_q) > stream_pairs(D) ? tile_bytes(D) : 0);

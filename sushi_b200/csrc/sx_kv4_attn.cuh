@@ -1,5 +1,5 @@
-// What the attention kernels over the 4-bit cache share: arguments, a request's geometry, the store
-// of an output row.
+// What the attention kernels over the 4-bit cache share: arguments, a request's geometry, scales of the
+// scores, the work lists.
 #pragma once
 
 #include "sx_kv4.cuh"

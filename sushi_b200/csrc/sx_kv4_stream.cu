@@ -29,9 +29,10 @@
 // into equal runs, one a CTA, so ragged lengths balance; a CTA's warps take its steps in turn, each
 // with its own ring of bulk copies.  A unit that several CTAs share is joined by sx_kv4_join.cu.
 //
-// Bound by HBM while all CTAs stream (5.4 to 6 TB/s), by the ALU instructions of the unpacking close behind
-// (571 a step of 32 keys; pipe 52% busy).  With the join: 64 requests of 1024 to 16384 keys and 8 key heads of
-// 128 (480 MB) 110 us, one of 131071 keys (151 MB) 48 us, one of 517 keys and 2 key heads 8.6 us.
+// Bound by instructions (633 a step of 32 keys, 56% of the issue slots, ALU pipe 50% busy), by HBM close behind (5 TB/s
+// while all CTAs stream).  With the join: 64 requests of 1024 to 16384 keys and 8 key heads of 128 (480 MB) 117 us, one
+// of 131071 keys (151 MB) 51 us, one of 517 keys and 2 key heads 9.1 us.  D = 256 with two column tiles runs at 255
+// registers and spills (208 bytes a thread, 280 in F16): 16 requests of 4 drafted tokens, 8 query heads a key head, 51 us.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 

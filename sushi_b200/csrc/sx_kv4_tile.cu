@@ -15,12 +15,12 @@
 // it by 2^8 (P's best at 2^7, at most 2^15).
 //
 // Precision.  bf16 calls round held keys and values, and P, to F16 once (11 bits): outputs are 4.6e-4 off beyond
-// their own rounding of 1.66e-3 (1.72e-3 in all).  F16 outputs would show it (4.5e-4 to 5.7e-4 in all, of 2.1e-4 of their
-// own), so F16 calls (FINE) keep each in two F16 parts, with a second product for the scores and two more for the values:
-// 2.08e-4 in all, for 1.1 to 1.7 times the time (a 4096-row chunk over 8192 keys 1072 us, 648 in bf16).  Sums are f32, cut (not rounded) at
-// each of the MMA's additions, so outputs come short with the tiles summed, in bf16 calls by 1.1e-4 over 131072 keys of
-// a CTA.  F16 calls, with three additions for one, sum at most MOST tiles in tensor memory and add them up in the
-// CTA's partial slot.
+// their own rounding of 1.66e-3 (1.72e-3 in all).  F16 outputs would show it (4.0e-4 to 5.7e-4 in all, of 2.1e-4
+// of their own), so F16 calls (FINE) keep each in two F16 parts, with a second product for the scores and two more
+// for the values: 2.08e-4 in all, for 1.1 to 1.7 times the time (4096 rows over 8192 keys 1100 us, 650 in bf16).
+// Sums are f32, cut (not rounded) at each of the MMA's additions, so outputs come short with the tiles summed, in
+// bf16 calls by 1.1e-4 over 131072 keys of a CTA.  F16 calls, with three additions for one, sum at most MOST tiles
+// in tensor memory and add them up in the CTA's partial slot.
 //
 // Work: the units' tiles laid end to end and cut into equal runs, one a CTA (one CTA an SM), so
 // causal lengths balance and few long rows are split; a unit of several CTAs is joined by
@@ -28,7 +28,7 @@
 //
 // Bound by the chain of a row tile: its softmax (2900 clocks a tile of 128 keys), then both row tiles'
 // products (3300), with the widening warps 4650 clocks busy beside them; 4096 rows over 8192 keys, 32 query and
-// 8 key heads of 128: 652 us with the join, 632 TFLOP/s.
+// 8 key heads of 128: 651 us with the join, 633 TFLOP/s.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 

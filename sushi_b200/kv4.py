@@ -188,9 +188,9 @@ _WS = {}  # (GPU, stream) -> _Kept
 def kv4_attention(q, cache: Kv4Cache, table, kv_lens, cu_q, max_q: int, scale=None, window: int = 0, out=None,
                   workspace=None):
     """sx_kv4_attention: q [tokens, heads, head_dim] (bf16/f16; channels contiguous) over the cache.
-    Request b's rows are cu_q[b]..cu_q[b+1] (at most max_q; a longer request's may come out NaN), its keys the kv_lens[b] tokens its row
-    of `table` [requests, width] names, the step's own last; causal, with a sliding window of
-    `window` positions when it is positive.  scale: head_dim**-0.5 when None.  out: an optional
+    Request b's rows are cu_q[b]..cu_q[b+1] (at most max_q; a longer request's may come out NaN), its
+    keys the kv_lens[b] tokens its row of `table` [requests, width] names, the step's own last; causal,
+    with a sliding window of `window` positions when it is positive.  scale: head_dim**-0.5 when None.  out: an optional
     contiguous tensor of q's shape and dtype.  workspace: an optional uint8 tensor of
     kv4_attention_workspace_bytes(...) bytes, for the calls of one stream by one host thread (without
     it, several threads may call on one stream)."""
